@@ -37,6 +37,7 @@ extern "C" {
 #define STMI_ACT_NONE 0
 #define STMI_ACT_RELU 1
 #define STMI_ACT_SIGMOID 2
+#define STMI_ACT_SILU 3 /* z * sigmoid(z); group norm only */
 
 /* which GEMM a packed weight buffer feeds */
 #define STMI_PACK_FWD 0   /* conv forward; transposed-conv backward-data */
@@ -361,6 +362,30 @@ int stmi_instance_norm_bwd_rows_count(int n, int h, int w, int c, int dtype);
 int stmi_instance_norm_param_grads(const float* rows, int nrows, int n, int c, float* dscale, float* dshift,
                                    int accumulate, void* stream);
 
+/* ---- group norm -------------------------------------------------------- */
+/* The instance norm's sibling with statistics over groups of neighbouring channels (no counterpart in the reference;
+ * groups == c is the instance norm, groups == 1 normalises a whole picture).  Group k of a sample is its channels
+ * k*c/groups .. (k+1)*c/groups - 1 at every pixel; with mean and variance over the group
+ *   xhat = (x - mean) / sqrt(var + eps),  y = act(scale[c] * xhat + shift[c]) [+ residual].
+ * c must be a multiple of groups and at most STMI_GN_MAX_C; every STMI_ACT_* activation; NaN and infinities of a group
+ * reach all of that group's outputs and no others.
+ *
+ * fwd : stats[n,groups,2] (fp32) = (mean, 1/sqrt(var + eps)), for the backward pass.  y may be x or residual itself.
+ * bwd : from dy (gradient w.r.t. y) to dx, and dscale[c], dshift[c] (fp32; written, or added to what they hold when
+ *       accumulate != 0; both NULL: not computed), summed over samples in a fixed order.  dx may be x or dy itself.  The
+ *       gradient w.r.t. residual is dy.  With n == 0, dscale and dshift are zero (left as they are when accumulated).
+ * ws  : scratch of stmi_group_norm_ws_floats floats, 16-byte aligned, for either call (NULL where that is 0).
+ * No float atomics: results are bit-reproducible, and a sample's result does not depend on the batch it is part of. */
+#define STMI_GN_MAX_C 8192
+long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype);
+int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps,
+                             const float* scale, const float* shift, const void* residual, void* y, int act,
+                             int n, int h, int w, int c, int groups, int dtype, void* stream);
+int stmi_group_norm_nhwc_bwd(const void* x, const void* dy, const float* stats,
+                             const float* scale, const float* shift,
+                             void* dx, float* dscale, float* dshift, int accumulate, float* ws,
+                             int act, int n, int h, int w, int c, int groups, int dtype, void* stream);
+
 /* ---- VGG pieces -------------------------------------------------------- */
 /* x*255/2 - mean                                    (vgg.py:11-17)
  * x fp32 [count/c, c] -> y in dtype; y = x*scale - mean[c]. */
@@ -437,6 +462,39 @@ int stmi_zero_multi(float* const* ptrs, const long* counts, int n, int* step_dev
 int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count,
                   float lr, float beta1, float beta2, float eps, float grad_scale,
                   int* step_dev, int t, void* stream);
+
+/* ---- gradient norm and clipping ----------------------------------------- */
+/* tf.clip_by_global_norm over any number of fp32 / bf16 tensors of any lengths, contiguous, at any element alignment
+ * (no call site in the reference, which trains unclipped):
+ *   norm = sqrt(sum over all tensors of sum(g^2)),  out = g * max_norm / max(norm, max_norm);
+ * a norm that is not finite makes every output NaN.  Squares are summed in double, in a fixed order.
+ * The tensors are described by a DEVICE table of chunks: stmi_grad_list_chunks gives its length, stmi_grad_list_fill
+ * writes it to HOST memory (no launch), the caller copies it to the device and keeps it for as long as the tensors
+ * (srcs) and the outputs (dsts, elementwise the same shapes and types; dsts[i] may be srcs[i], no other overlap) stay
+ * where they are.  Tensors of length zero have no chunks.
+ * ws: STMI_GRAD_WS_DOUBLES doubles of scratch; a call overwrites it entirely.  Calls that share a ws must be ordered.
+ * stmi_grad_sum_squares : leaves partial sums of squares in ws for stmi_adam_tf1_clip.
+ * stmi_grad_norm        : the same, and norm (device fp32 [1]).
+ * stmi_grad_clip        : the same, and the outputs; norm (may be NULL) is the norm BEFORE clipping.  Where dsts[i] is
+ *                         srcs[i] and nothing is to be clipped, nothing is written.  max_norm: finite, > 0. */
+#define STMI_GRAD_WS_DOUBLES 2048
+typedef struct {
+    const void* src;
+    void* dst;
+    int count, dtype;
+} stmi_grad_chunk;
+long stmi_grad_list_chunks(const long* counts, int n);
+int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
+                        stmi_grad_chunk* host_table);
+int stmi_grad_sum_squares(const stmi_grad_chunk* table, int nchunks, double* ws, void* stream);
+int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float* norm, void* stream);
+int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream);
+/* stmi_adam_tf1 of gradients clipped on the way in: g * grad_scale is scaled by max_norm / max(norm, max_norm) with
+ * norm = |grad_scale| * sqrt(sum of the partial sums in ws), as stmi_grad_sum_squares left them for all gradients that
+ * share the norm.  norm (device fp32 [1], may be NULL) receives it. */
+int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count,
+                       float lr, float beta1, float beta2, float eps, float grad_scale,
+                       const double* ws, float max_norm, float* norm, int* step_dev, int t, void* stream);
 
 /* ---- row patches for layers with < 8 channels on one side (the 9x9 RGB layers) ----------
  * A kw x c window of an NHWC tensor is kw*c contiguous elements.  Copying it once per pixel

@@ -107,6 +107,12 @@ int in_apply_impl(const void* x, const float* stats, const float* scale, const f
 int in_bwd_impl(const void* x, const void* dy, const float* stats, const float* scale, const float* shift, void* dx,
                 float* dscale, float* dshift, int accumulate, float* ws, int act, int n, int h, int w, int c, int dtype,
                 hipStream_t s);
+long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype);
+int gn_fwd_impl(const void* x, float* ws, float* stats, float eps, const float* scale, const float* shift,
+                const void* residual, void* y, int act, int n, int h, int w, int c, int groups, int dtype, hipStream_t s);
+int gn_bwd_impl(const void* x, const void* dy, const float* stats, const float* scale, const float* shift, void* dx,
+                float* dscale, float* dshift, int accumulate, float* ws, int act, int n, int h, int w, int c, int groups,
+                int dtype, hipStream_t s);
 int scale_shift_impl(const float*, const float*, void*, float, long, int, int, hipStream_t);
 int cast_impl(const void*, void*, long, int, int, hipStream_t);
 int clip_impl(float*, long, float, float, hipStream_t);
@@ -121,6 +127,14 @@ int gram_mse_impl(const float*, const float*, void*, float*, float, float, int, 
 int tv_impl(const float*, void*, float*, float, int, int, int, int, int, hipStream_t);
 int loss_slots_sum_impl(const float* slots, const int* first, int nterms, float* out, hipStream_t s);
 int adam_impl(float*, const float*, float*, float*, long, float, float, float, float, float, int*, int, hipStream_t);
+long grad_list_chunks(const long* counts, int n);
+void grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
+                    stmi_grad_chunk* table);
+int grad_squares_impl(const stmi_grad_chunk* table, int nchunks, double* ws, hipStream_t s);
+int grad_norm_impl(const double* ws, float* norm, hipStream_t s);
+int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws, float max_norm, float* norm, hipStream_t s);
+int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, float lr, float b1, float b2, float eps,
+                   float grad_scale, const double* ws, float max_norm, float* norm, int* step_dev, int t, hipStream_t s);
 
 static int check_dtype(int dtype) {
     if (dtype == STMI_F32 || dtype == STMI_BF16) return STMI_OK;
@@ -573,6 +587,39 @@ int stmi_instance_norm_param_grads(const float* rows, int nrows, int n, int c, f
     return in_param_grads_impl(rows, nrows, n, c, dscale, dshift, accumulate, S(stream));
 }
 
+static int check_group_norm(const char* who, int act, int n, int h, int w, int c, int groups, int dtype) {
+    if (check_dtype(dtype)) return STMI_ERR_INVALID;
+    STMI_REQUIRE(n >= 0 && h > 0 && w > 0 && c > 0 && groups > 0, "%s: bad arguments", who);
+    STMI_REQUIRE(c % groups == 0, "%s: %d channels are no multiple of %d groups", who, c, groups);
+    STMI_REQUIRE(c <= STMI_GN_MAX_C, "%s: more than %d channels (got %d)", who, STMI_GN_MAX_C, c);
+    STMI_REQUIRE((long)h * w < (1L << 31), "%s: 2^31 pixels or more in a sample", who);
+    STMI_REQUIRE(act >= STMI_ACT_NONE && act <= STMI_ACT_SILU, "%s: bad activation %d", who, act);
+    return STMI_OK;
+}
+
+long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype) {
+    if (check_group_norm("group_norm_ws_floats", STMI_ACT_NONE, n, h, w, c, groups, dtype)) return -1;
+    return gn_ws_floats(n, h, w, c, groups, dtype);
+}
+
+int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps, const float* scale, const float* shift,
+                             const void* residual, void* y, int act, int n, int h, int w, int c, int groups, int dtype,
+                             void* stream) {
+    if (check_group_norm("group_norm_nhwc_fwd", act, n, h, w, c, groups, dtype)) return STMI_ERR_INVALID;
+    if (n == 0) return STMI_OK;
+    STMI_REQUIRE(x && ws && stats && scale && shift && y, "group_norm_nhwc_fwd: bad arguments");
+    return gn_fwd_impl(x, ws, stats, eps, scale, shift, residual, y, act, n, h, w, c, groups, dtype, S(stream));
+}
+
+int stmi_group_norm_nhwc_bwd(const void* x, const void* dy, const float* stats, const float* scale, const float* shift,
+                             void* dx, float* dscale, float* dshift, int accumulate, float* ws, int act, int n, int h, int w,
+                             int c, int groups, int dtype, void* stream) {
+    if (check_group_norm("group_norm_nhwc_bwd", act, n, h, w, c, groups, dtype)) return STMI_ERR_INVALID;
+    STMI_REQUIRE((n == 0 || (x && dy && stats && scale && shift && dx && ws)) && (dscale == nullptr) == (dshift == nullptr),
+                 "group_norm_nhwc_bwd: bad arguments");
+    return gn_bwd_impl(x, dy, stats, scale, shift, dx, dscale, dshift, accumulate, ws, act, n, h, w, c, groups, dtype, S(stream));
+}
+
 int stmi_scale_shift(const float* x, const float* mean, void* y, float scale, long count, int c, int dtype,
                      void* stream) {
     if (check_dtype(dtype)) return STMI_ERR_INVALID;
@@ -675,6 +722,56 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count, floa
     STMI_REQUIRE(step_dev || t >= 1, "adam_tf1: step t must be >= 1 (got %d)", t);
     if (count == 0) return STMI_OK;
     return adam_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, step_dev, t, S(stream));
+}
+
+long stmi_grad_list_chunks(const long* counts, int n) {
+    if (!counts && n > 0) return -1;
+    for (int i = 0; i < n; i++)
+        if (counts[i] < 0) return -1;
+    return grad_list_chunks(counts, n);
+}
+
+int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
+                        stmi_grad_chunk* host_table) {
+    STMI_REQUIRE(n >= 0 && (n == 0 || (srcs && dsts && counts && dtypes)), "grad_list_fill: bad arguments");
+    for (int i = 0; i < n; i++) {
+        if (check_dtype(dtypes[i])) return STMI_ERR_INVALID;
+        STMI_REQUIRE(counts[i] >= 0 && (counts[i] == 0 || (srcs[i] && dsts[i])), "grad_list_fill: bad tensor %d", i);
+        const uintptr_t size = dtypes[i] == STMI_BF16 ? 2 : 4;
+        STMI_REQUIRE((uintptr_t)srcs[i] % size == 0 && (uintptr_t)dsts[i] % size == 0, "grad_list_fill: tensor %d is not aligned to its elements", i);
+    }
+    const long chunks = grad_list_chunks(counts, n);
+    STMI_REQUIRE(chunks == 0 || host_table, "grad_list_fill: null table");
+    STMI_REQUIRE(chunks < (1L << 31), "grad_list_fill: more than 2^31 chunks");
+    grad_list_fill(srcs, dsts, counts, dtypes, n, host_table);
+    return STMI_OK;
+}
+
+int stmi_grad_sum_squares(const stmi_grad_chunk* table, int nchunks, double* ws, void* stream) {
+    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws, "grad_sum_squares: bad arguments");
+    return grad_squares_impl(table, nchunks, ws, S(stream));
+}
+
+int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float* norm, void* stream) {
+    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws && norm, "grad_norm: bad arguments");
+    const int rc = grad_squares_impl(table, nchunks, ws, S(stream));
+    return rc ? rc : grad_norm_impl(ws, norm, S(stream));
+}
+
+int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream) {
+    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws, "grad_clip: bad arguments");
+    STMI_REQUIRE(max_norm > 0.f && max_norm <= 3.402823466e38f, "grad_clip: max_norm must be finite and > 0 (got %g)", (double)max_norm);
+    const int rc = grad_squares_impl(table, nchunks, ws, S(stream));
+    return rc ? rc : grad_scale_impl(table, nchunks, ws, max_norm, norm, S(stream));
+}
+
+int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count, float lr, float beta1, float beta2,
+                       float eps, float grad_scale, const double* ws, float max_norm, float* norm, int* step_dev, int t,
+                       void* stream) {
+    STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws, "adam_tf1_clip: bad arguments");
+    STMI_REQUIRE(step_dev || t >= 1, "adam_tf1_clip: step t must be >= 1 (got %d)", t);
+    STMI_REQUIRE(max_norm > 0.f && max_norm <= 3.402823466e38f, "adam_tf1_clip: max_norm must be finite and > 0 (got %g)", (double)max_norm);
+    return adam_clip_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, ws, max_norm, norm, step_dev, t, S(stream));
 }
 
 int stmi_cast(const void* src, void* dst, long count, int dtype, int to_f32, void* stream) {

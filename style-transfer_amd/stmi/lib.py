@@ -11,9 +11,10 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('STMI_LIB_PATH') or os.path.join(_HERE, '..', 'libstmi355.so')   # STMI_LIB_PATH: tuning builds
 
 F32, BF16 = 0, 1
-ACT_NONE, ACT_RELU, ACT_SIGMOID = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3
 PACK_FWD, PACK_DGRAD, PACK_FWD_ROWOUT, PACK_FWD_RGB, PACK_DGRAD_RGB = 0, 1, 2, 3, 4
 LOSS_SLOT_FLOATS, LOSS_TERMS_MAX = 1024, 8
+GN_MAX_C, GRAD_WS_DOUBLES = 8192, 2048
 
 _c_int, _c_long, _c_float, _vp = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p
 
@@ -70,6 +71,9 @@ SIGNATURES = {
     'stmi_instance_norm_nhwc_bwd_rows': (_c_int, [_vp] * 8 + [_c_int, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_instance_norm_bwd_rows_count': (_c_int, [_c_int] * 5),
     'stmi_instance_norm_param_grads': (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp]),
+    'stmi_group_norm_ws_floats': (_c_long, [_c_int] * 6),
+    'stmi_group_norm_nhwc_fwd': (_c_int, [_vp, _vp, _vp, _c_float] + [_vp] * 4 + [_c_int] * 7 + [_vp]),
+    'stmi_group_norm_nhwc_bwd': (_c_int, [_vp] * 8 + [_c_int, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_scale_shift': (_c_int, [_vp, _vp, _vp, _c_float, _c_long, _c_int, _c_int, _vp]),
     'stmi_maxpool2x2_same_fwd': (_c_int, [_vp, _vp] + [_c_int] * 5 + [_vp]),
     'stmi_maxpool2x2_same_bwd': (_c_int, [_vp, _vp, _vp] + [_c_int] * 5 + [_vp]),
@@ -84,6 +88,12 @@ SIGNATURES = {
     'stmi_tv_loss_fwd_bwd': (_c_int, [_vp] * 3 + [_c_float] + [_c_int] * 5 + [_vp]),
     'stmi_loss_slots_sum': (_c_int, [_vp, _vp, _c_int, _vp, _vp]),
     'stmi_adam_tf1': (_c_int, [_vp] * 4 + [_c_long] + [_c_float] * 5 + [_vp, _c_int, _vp]),
+    'stmi_grad_list_chunks': (_c_long, [_vp, _c_int]),
+    'stmi_grad_list_fill': (_c_int, [_vp] * 4 + [_c_int, _vp]),
+    'stmi_grad_sum_squares': (_c_int, [_vp, _c_int, _vp, _vp]),
+    'stmi_grad_norm': (_c_int, [_vp, _c_int] + [_vp] * 3),
+    'stmi_grad_clip': (_c_int, [_vp, _c_int, _vp, _c_float, _vp, _vp]),
+    'stmi_adam_tf1_clip': (_c_int, [_vp] * 4 + [_c_long] + [_c_float] * 5 + [_vp, _c_float, _vp, _vp, _c_int, _vp]),
     'stmi_cast': (_c_int, [_vp, _vp, _c_long, _c_int, _c_int, _vp]),
     'stmi_pixels_to_rows': (_c_int, [_vp, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_rows_to_pixels_sum': (_c_int, [_vp, _vp, _vp] + [_c_int] * 7 + [_vp]),
@@ -98,6 +108,11 @@ class PackDesc(ctypes.Structure):
     """stmi_pack_desc of include/stmi.h"""
     _fields_ = [('src_off', _c_long), ('dst_off', _c_long), ('kh', _c_int), ('kw', _c_int), ('ci', _c_int),
                 ('co', _c_int), ('mode', _c_int), ('reserved', _c_int)]
+
+
+class GradChunk(ctypes.Structure):
+    """stmi_grad_chunk of include/stmi.h"""
+    _fields_ = [('src', _vp), ('dst', _vp), ('count', _c_int), ('dtype', _c_int)]
 
 
 _lib = None

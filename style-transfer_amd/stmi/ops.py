@@ -8,7 +8,7 @@ Tensors are NHWC, contiguous, on the current HIP device, float32 or bfloat16.
 import torch
 
 from . import lib as _lib
-from .lib import ACT_NONE, ACT_RELU, ACT_SIGMOID, PACK_DGRAD, PACK_DGRAD_RGB, PACK_FWD, PACK_FWD_RGB, PACK_FWD_ROWOUT  # noqa: F401
+from .lib import ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, PACK_DGRAD, PACK_DGRAD_RGB, PACK_FWD, PACK_FWD_RGB, PACK_FWD_ROWOUT  # noqa: F401
 
 _DT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
@@ -706,6 +706,87 @@ def instance_norm_bwd(x, dy, stats, scale, shift, dscale, dshift, act=ACT_NONE, 
     return dx
 
 
+# ------------------------------------------------------------- group norm
+def _chk_here(t, name):
+    """The launch goes to the current device's current stream: a tensor of another device would be read there."""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError('%s lives on %s, not on the current device cuda:%d' % (name, t.device, torch.cuda.current_device()))
+
+
+def _chk_out(out, name, like, *exact):
+    """An output buffer of like's shape and type: one of `exact` itself, or no overlap with any of them."""
+    _chk(out, name, like.dtype, like.shape)
+    a, size = out.data_ptr(), out.numel() * out.element_size()
+    for t in exact:
+        if t is not None and t.data_ptr() != a and abs(t.data_ptr() - a) < size:
+            raise ValueError('%s overlaps an input without being the same tensor' % name)
+    return out
+
+
+def group_norm_ws(n, h, w, c, groups, dtype, device):
+    """Workspace of group_norm_fwd / group_norm_bwd for this geometry."""
+    if dtype not in _DT:
+        raise TypeError('stmi ops take float32 or bfloat16 tensors, got %s' % dtype)
+    need = _lib.load().stmi_group_norm_ws_floats(n, h, w, c, groups, _DT[dtype])
+    if need < 0:
+        raise _lib.StmiError(_lib.load().stmi_last_error().decode())
+    return torch.empty(max(need, 4), dtype=torch.float32, device=device)
+
+
+def _group_norm_ws(ws, x, groups):
+    n, h, w, c = x.shape
+    if ws is None:
+        return group_norm_ws(n, h, w, c, groups, x.dtype, x.device)
+    _chk(ws, 'ws', torch.float32)
+    if ws.numel() < _lib.load().stmi_group_norm_ws_floats(n, h, w, c, groups, _dt(x)) or ws.data_ptr() % 16:
+        raise ValueError('ws must be 16-byte aligned and hold group_norm_ws(...) floats')
+    return ws
+
+
+def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None, out=None, stats=None, eps=IN_EPS):
+    """y = act(scale * xhat + shift) [+ residual], normalised over `groups` groups of neighbouring channels of x [n,h,w,c].
+    Returns (y, stats); stats [n,groups,2] = (mean, 1/sqrt(var+eps)) for group_norm_bwd.  out may be x or residual itself;
+    any other overlap is not allowed.  act: ACT_NONE, ACT_RELU, ACT_SIGMOID or ACT_SILU."""
+    n, h, w, c = x.shape
+    _chk(x, 'x')
+    _chk_here(x, 'x')
+    _chk(scale, 'scale', torch.float32, (c,))
+    _chk(shift, 'shift', torch.float32, (c,))
+    if residual is not None:
+        _chk(residual, 'residual', x.dtype, x.shape)
+    y = torch.empty_like(x) if out is None else _chk_out(out, 'out', x, x, residual)
+    ws = _group_norm_ws(ws, x, groups)
+    if stats is None:
+        stats = torch.empty((n, groups, 2), dtype=torch.float32, device=x.device)
+    else:
+        _chk(stats, 'stats', torch.float32, (n, groups, 2))
+    _lib.call('stmi_group_norm_nhwc_fwd', x.data_ptr(), ws.data_ptr(), stats.data_ptr(), float(eps), scale.data_ptr(),
+              shift.data_ptr(), _ptr(residual), y.data_ptr(), act, n, h, w, c, groups, _dt(x), _stream())
+    return y, stats
+
+
+def group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, act=ACT_NONE, ws=None, out=None, accumulate=True):
+    """dx returned; parameter gradients are ADDED into dscale/dshift (fp32 [c]), or WRITTEN when accumulate is False;
+    both None: not computed.  stats: what group_norm_fwd returned for x.  The gradient of a residual is dy.  out may be x or
+    dy itself; any other overlap is not allowed."""
+    n, h, w, c = x.shape
+    _chk(x, 'x')
+    _chk_here(x, 'x')
+    _chk(dy, 'dy', x.dtype, x.shape)
+    _chk(stats, 'stats', torch.float32, (n, groups, 2))
+    if (dscale is None) != (dshift is None):
+        raise ValueError('dscale and dshift are given together or not at all')
+    for t, nm in ((scale, 'scale'), (shift, 'shift'), (dscale, 'dscale'), (dshift, 'dshift')):
+        if t is not None:
+            _chk(t, nm, torch.float32, (c,))
+    ws = _group_norm_ws(ws, x, groups)
+    dx = torch.empty_like(x) if out is None else _chk_out(out, 'out', x, x, dy)
+    _lib.call('stmi_group_norm_nhwc_bwd', x.data_ptr(), dy.data_ptr(), stats.data_ptr(), scale.data_ptr(), shift.data_ptr(),
+              dx.data_ptr(), _ptr(dscale), _ptr(dshift), int(accumulate), ws.data_ptr(), act, n, h, w, c, groups, _dt(x),
+              _stream())
+    return dx
+
+
 # -------------------------------------------------------------- VGG pieces
 def scale_shift(x_f32, mean, scale, dtype, out=None):
     _chk(x_f32, 'x', torch.float32)
@@ -863,17 +944,114 @@ def tv_loss_fwd_bwd(img_f32, loss, weight, dtype, out=None):
     return grad
 
 
+# ------------------------------------------------- gradient norm, clipping
+def _chk_disjoint(tensors, outs):
+    """An output may be its own tensor; any other overlap of an output with a tensor or an output is refused: chunks are
+    read and written in no order."""
+    spans = []
+    for i, (t, o) in enumerate(zip(tensors, outs)):
+        if t.numel():
+            nbytes = t.numel() * t.element_size()
+            spans.append((t.data_ptr(), t.data_ptr() + nbytes, 0, i))
+            spans.append((o.data_ptr(), o.data_ptr() + nbytes, 1, i))
+    reach = [(0, -1), (0, -1)]          # the two tensors that reach furthest so far, of different indexes
+    last = (0, 0, -1)                   # the output that reaches furthest so far (outputs are disjoint)
+    for start, end, is_out, i in sorted(spans):
+        if is_out:
+            clash = last[1] > start
+            for e, j in reach:
+                clash = clash or (e > start and j != i)
+            clash = clash or any(e > start and j == i for e, j in reach) and tensors[i].data_ptr() != start
+            last = (start, end, i)
+        else:
+            clash = last[1] > start and not (last[2] == i and last[0] == start)
+            reach = sorted(reach + [(end, i)], reverse=True)[:2]
+        if clash:
+            raise ValueError('output or tensor %d overlaps another one' % i)
+
+
+class GradList:
+    """The gradients of a training step as ONE list: their global norm, and clipping by it, in one launch each however
+    many there are.  tensors: contiguous fp32 / bf16 tensors of any lengths on the current device; outs: what clip() writes,
+    tensor by tensor (default: the tensors themselves).  The list keeps the tensors, their places (a device table built
+    here, once) and a workspace: build it before a graph that uses it is captured, keep it as long as the graph, and order
+    its calls (two graphs that may run at the same time need a list each)."""
+
+    def __init__(self, tensors, outs=None):
+        import ctypes
+        tensors = list(tensors)
+        outs = tensors if outs is None else list(outs)
+        if len(outs) != len(tensors):
+            raise ValueError('%d tensors, but %d outputs' % (len(tensors), len(outs)))
+        for i, (t, o) in enumerate(zip(tensors, outs)):
+            _dt(_chk(t, 'tensor %d' % i))
+            _chk_here(t, 'tensor %d' % i)
+            _chk(o, 'output %d' % i, t.dtype, t.shape)
+            _chk_here(o, 'output %d' % i)
+        _chk_disjoint(tensors, outs)
+        self._keep = (tensors, outs)
+        self.device = torch.device('cuda', torch.cuda.current_device())
+        n, h = len(tensors), _lib.load()
+        counts = (ctypes.c_long * n)(*[t.numel() for t in tensors])
+        self._n = h.stmi_grad_list_chunks(counts, n)
+        table = (_lib.GradChunk * max(self._n, 1))()
+        _lib.call('stmi_grad_list_fill', (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
+                  (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts,
+                  (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors]), n, table)
+        self._table = torch.frombuffer(table, dtype=torch.uint8).to(self.device)
+        self._ws = torch.empty(_lib.GRAD_WS_DOUBLES, dtype=torch.float64, device=self.device)
+
+    def _norm_out(self, out):
+        _chk_here(self._table, 'the list')
+        if out is None:
+            return torch.empty(1, dtype=torch.float32, device=self.device)
+        return _chk(out, 'norm', torch.float32, (1,))
+
+    def sum_squares(self):
+        """Leaves the sum of squares (as partial sums) for adam_tf1(..., clip=self)."""
+        _chk_here(self._table, 'the list')
+        _lib.call('stmi_grad_sum_squares', self._table.data_ptr(), self._n, self._ws.data_ptr(), _stream())
+
+    def norm(self, out=None):
+        """The global L2 norm, fp32 [1] on the device."""
+        out = self._norm_out(out)
+        _lib.call('stmi_grad_norm', self._table.data_ptr(), self._n, self._ws.data_ptr(), out.data_ptr(), _stream())
+        return out
+
+    def clip(self, max_norm, norm=None):
+        """outs = tensors * max_norm / max(norm, max_norm); returns the norm before clipping, fp32 [1] on the device.  A norm
+        that is not finite makes every output NaN."""
+        norm = self._norm_out(norm)
+        _lib.call('stmi_grad_clip', self._table.data_ptr(), self._n, self._ws.data_ptr(), float(max_norm), norm.data_ptr(),
+                  _stream())
+        return norm
+
+
 # -------------------------------------------------------------- optimizer
-def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, step_dev=None, t=0, advance=True):
+def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, step_dev=None, t=0, advance=True, clip=None,
+             max_norm=None, norm=None):
     """TF1 Adam.  With `step_dev` (int32 [1] on the device) the step number lives on the device, which
     makes the call replayable inside a HIP graph: advance=True increments it before use; advance=False
-    uses it as it stands (a second slice of the same parameter set in the same step)."""
+    uses it as it stands (a second slice of the same parameter set in the same step).
+    clip: a GradList whose sum_squares() has been launched; the gradients g * grad_scale are then clipped to the global
+    norm max_norm on their way in, with |grad_scale| times the list's norm (fp32 [1] `norm` receives it)."""
+    if (clip is None) != (max_norm is None) or (clip is None and norm is not None):
+        raise ValueError('clip and max_norm are given together, norm with them')
     for tns, nm in ((p, 'p'), (g, 'g'), (m, 'm'), (v, 'v')):
         _chk(tns, nm, torch.float32)
         assert tns.numel() == p.numel()
     if step_dev is not None:
         _chk(step_dev, 'step_dev', torch.int32)
         t = 0 if advance else -1
+    if clip is not None:
+        _chk_here(p, 'p')
+        _chk_here(clip._table, 'clip')
+        if norm is not None:
+            _chk(norm, 'norm', torch.float32, (1,))
+        _lib.call('stmi_adam_tf1_clip', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
+                  float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws.data_ptr(), float(max_norm), _ptr(norm),
+                  _ptr(step_dev), int(t), _stream())
+        return
     _lib.call('stmi_adam_tf1', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
               float(beta1), float(beta2), float(eps), float(grad_scale), _ptr(step_dev), int(t), _stream())
 

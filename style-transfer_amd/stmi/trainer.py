@@ -114,7 +114,10 @@ class GradBuckets:
 class StyleTrainer:
     def __init__(self, batch, height, width, device, vgg_weights, vgg_mean, style_weight, content_weight, tv_weight,
                  dtype=torch.float32, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, params=None, seed=1,
-                 world_size=1, group=None, use_graph=True):
+                 world_size=1, group=None, use_graph=True, max_grad_norm=None):
+        """max_grad_norm: clip the gradients of all 48 variables (averaged over the ranks) to this global norm before the
+        update, as tf.clip_by_global_norm does; grad_norm then holds the norm before clipping.  None: no clipping, as in
+        the reference."""
         self.n, self.h, self.w, self.device, self.dtype = batch, height, width, device, dtype
         self.sw, self.cw, self.tvw = style_weight, content_weight, tv_weight
         self.lr, self.b1, self.b2, self.eps = lr, beta1, beta2, eps
@@ -142,6 +145,13 @@ class StyleTrainer:
         self.v = torch.zeros_like(self.net.flat)
         self.step_dev = torch.zeros(1, dtype=torch.int32, device=device)
         self.style_targets = None
+        self.max_grad_norm = max_grad_norm
+        self.grad_list = self.grad_norm = None
+        if max_grad_norm is not None:
+            if not 0 < max_grad_norm < float('inf'):
+                raise ValueError('max_grad_norm must be finite and > 0, got %r' % (max_grad_norm,))
+            self.grad_list = ops.GradList([self.net.flat_grad])
+            self.grad_norm = torch.zeros(1, dtype=torch.float32, device=device)
         self.buckets = None
         if world_size > 1:
             self.buckets = GradBuckets(self.net.flat_grad, [self.net.param_range(hi, lo) for hi, lo in BWD_SEGMENTS],
@@ -203,10 +213,16 @@ class StyleTrainer:
         return d_out
 
     def _adam(self, lo=0, hi=None, advance=True):
-        """TF1 Adam on flat[lo:hi]; the step counter was advanced by the launch that cleared the accumulators."""
+        """TF1 Adam on flat[lo:hi]; the step counter was advanced by the launch that cleared the accumulators.
+        advance: the first call of a step; with clipping it needs every gradient of the step."""
         sl = slice(lo, hi)
+        clip = {}
+        if self.grad_list is not None:
+            if advance:
+                self.grad_list.sum_squares()
+            clip = dict(clip=self.grad_list, max_norm=self.max_grad_norm, norm=self.grad_norm)
         ops.adam_tf1(self.net.flat[sl], self.net.flat_grad[sl], self.m[sl], self.v[sl], self.lr, self.b1, self.b2,
-                     self.eps, grad_scale=1.0 / self.world, step_dev=self.step_dev, advance=False)
+                     self.eps, grad_scale=1.0 / self.world, step_dev=self.step_dev, advance=False, **clip)
 
     def _update(self):
         self._adam()
@@ -241,7 +257,9 @@ class StyleTrainer:
 
     def _before(self, i):
         nb = len(BWD_SEGMENTS)
-        if i >= nb:
+        if i == nb and self.grad_list is not None:
+            self.buckets.wait()                    # the norm needs every bucket
+        elif i >= nb:
             self.buckets.wait_bucket(i - nb)       # Adam of bucket i - nb needs that bucket only
 
     def _run_eager(self):
