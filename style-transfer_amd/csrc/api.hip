@@ -592,7 +592,7 @@ static int check_group_norm(const char* who, int act, int n, int h, int w, int c
     STMI_REQUIRE(n >= 0 && h > 0 && w > 0 && c > 0 && groups > 0, "%s: bad arguments", who);
     STMI_REQUIRE(c % groups == 0, "%s: %d channels are no multiple of %d groups", who, c, groups);
     STMI_REQUIRE(c <= STMI_GN_MAX_C, "%s: more than %d channels (got %d)", who, STMI_GN_MAX_C, c);
-    STMI_REQUIRE((long)h * w < (1L << 31), "%s: 2^31 pixels or more in a sample", who);
+    STMI_REQUIRE((long)h * w <= (1L << 31) - (1L << 16), "%s: more than 2^31 - 2^16 pixels in a sample", who);
     STMI_REQUIRE(act >= STMI_ACT_NONE && act <= STMI_ACT_SILU, "%s: bad activation %d", who, act);
     return STMI_OK;
 }
