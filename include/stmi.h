@@ -374,10 +374,10 @@ int stmi_instance_norm_param_grads(const float* rows, int nrows, int n, int c, f
  * bwd : from dy (gradient w.r.t. y) to dx, and dscale[c], dshift[c] (fp32; written, or added to what they hold when
  *       accumulate != 0; both NULL: not computed), summed over samples in a fixed order.  dx may be x or dy itself.  The
  *       gradient w.r.t. residual is dy.  With n == 0, dscale and dshift are zero (left as they are when accumulated).
- * ws  : scratch of stmi_group_norm_ws_floats floats, 16-byte aligned, for either call (NULL where that is 0).
+ * ws  : scratch of stmi_group_norm_ws_floats floats for the direction, 16-byte aligned (NULL where that is 0).
  * No float atomics: results are bit-reproducible, and a sample's result does not depend on the batch it is part of. */
-#define STMI_GN_MAX_C 8192
-long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype);
+#define STMI_GN_MAX_C 4096
+long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward);
 int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps,
                              const float* scale, const float* shift, const void* residual, void* y, int act,
                              int n, int h, int w, int c, int groups, int dtype, void* stream);

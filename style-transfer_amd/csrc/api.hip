@@ -107,7 +107,7 @@ int in_apply_impl(const void* x, const float* stats, const float* scale, const f
 int in_bwd_impl(const void* x, const void* dy, const float* stats, const float* scale, const float* shift, void* dx,
                 float* dscale, float* dshift, int accumulate, float* ws, int act, int n, int h, int w, int c, int dtype,
                 hipStream_t s);
-long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype);
+long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward);
 int gn_fwd_impl(const void* x, float* ws, float* stats, float eps, const float* scale, const float* shift,
                 const void* residual, void* y, int act, int n, int h, int w, int c, int groups, int dtype, hipStream_t s);
 int gn_bwd_impl(const void* x, const void* dy, const float* stats, const float* scale, const float* shift, void* dx,
@@ -597,9 +597,9 @@ static int check_group_norm(const char* who, int act, int n, int h, int w, int c
     return STMI_OK;
 }
 
-long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype) {
+long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward) {
     if (check_group_norm("group_norm_ws_floats", STMI_ACT_NONE, n, h, w, c, groups, dtype)) return -1;
-    return gn_ws_floats(n, h, w, c, groups, dtype);
+    return n == 0 ? 0 : gn_ws_floats(n, h, w, c, groups, dtype, backward);
 }
 
 int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps, const float* scale, const float* shift,
@@ -607,7 +607,8 @@ int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps, 
                              void* stream) {
     if (check_group_norm("group_norm_nhwc_fwd", act, n, h, w, c, groups, dtype)) return STMI_ERR_INVALID;
     if (n == 0) return STMI_OK;
-    STMI_REQUIRE(x && ws && stats && scale && shift && y, "group_norm_nhwc_fwd: bad arguments");
+    STMI_REQUIRE(x && stats && scale && shift && y && (ws || gn_ws_floats(n, h, w, c, groups, dtype, 0) == 0),
+                 "group_norm_nhwc_fwd: bad arguments");
     return gn_fwd_impl(x, ws, stats, eps, scale, shift, residual, y, act, n, h, w, c, groups, dtype, S(stream));
 }
 
@@ -615,7 +616,7 @@ int stmi_group_norm_nhwc_bwd(const void* x, const void* dy, const float* stats, 
                              void* dx, float* dscale, float* dshift, int accumulate, float* ws, int act, int n, int h, int w,
                              int c, int groups, int dtype, void* stream) {
     if (check_group_norm("group_norm_nhwc_bwd", act, n, h, w, c, groups, dtype)) return STMI_ERR_INVALID;
-    STMI_REQUIRE((n == 0 || (x && dy && stats && scale && shift && dx && ws)) && (dscale == nullptr) == (dshift == nullptr),
+    STMI_REQUIRE((n == 0 || (x && dy && stats && scale && shift && dx && (ws || gn_ws_floats(n, h, w, c, groups, dtype, 1) == 0))) && (dscale == nullptr) == (dshift == nullptr),
                  "group_norm_nhwc_bwd: bad arguments");
     return gn_bwd_impl(x, dy, stats, scale, shift, dx, dscale, dshift, accumulate, ws, act, n, h, w, c, groups, dtype, S(stream));
 }

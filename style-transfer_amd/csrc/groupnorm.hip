@@ -8,31 +8,53 @@
 //   dx = rstd * (scale_c g - m1 - xhat * m2),  m1 = sum(scale_c g) / M,  m2 = sum(scale_c g xhat) / M over the group
 //
 // Two launches a direction: a reduction over slices of the samples leaves one partial result per slice and group, and the
-// blocks of the second launch fold the partials of their sample and stream the tensor once more.
+// blocks of the second launch fold the partials of their sample and stream the tensor once more.  Samples whose groups fit
+// the registers of a block take one launch (at the end of the file).
 //
 // Layout of the work: a sample is a flat run of P * C elements, cut into rows of L = lcm(C, V) elements (V: the elements
 // of a 16-byte access), so that a thread that owns one 16-byte column of a row sees the SAME V channels in every row
 // whatever C is.  What does not fill a row behind the last one is the tail; it belongs to the last slice.  The cut depends
 // on the sample's own size alone, and accesses need only the elements' alignment (global memory takes 16-byte accesses at
 // any address): a sample's bits depend neither on its batch nor on its place.
-// Statistics are merged as (count, mean, sum of squared deviations) with the means of the parts (Chan et al.): no
-// cancellation however large the mean is next to the deviation.  Sums are fp32, no atomics: bit-reproducible.
+// A mean is formed first and deviations from it are summed then, within a batch of loads, over a block's threads and over
+// the slices: no cancellation however large the mean is next to the deviation.  Sums are fp32, no atomics:
+// bit-reproducible.
+// What the launches of small tensors cost is instructions, not bytes: divisions by the geometry's numbers are done by the
+// host (gn_div), constants of the channels come from a table in shared memory that a block makes once, reductions over
+// lanes use DPP.
 #include "common.hpp"
 
 #include <type_traits>
 
 namespace stmi {
 
-constexpr int kGnT = 512;      // threads of a block
-constexpr int kGnSlices = 512; // most slices of a sample
-constexpr int kGnFold = 8192;  // partials (slices x groups) of a sample that the apply blocks fold themselves
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+
+constexpr int kGnT = 512;        // threads of a block
+constexpr int kGnSlices = 512;   // most slices of a sample (64 lanes of kGnFoldLane fold them)
+constexpr int kGnFoldLane = 8;   // partials a lane folds
+constexpr int kGnUnitFwd = 1024, kGnUnitBwd = 512;   // most threads of a unit's block
 
 struct GnGeom {
     int N, P, C, G, D;
-    int L, Q, R;     // elements and V-wide columns of a row, whole rows of a sample
-    int QT, tiles;   // columns a block owns, blocks side by side in a row
-    int S, rows;     // slices of a sample, rows of a slice
+    int L, Q, R;         // elements and V-wide columns of a row, whole rows of a sample
+    int QT, tiles;       // columns a block owns, blocks side by side in a row
+    int S, rows;         // slices of a sample, rows of a slice
+    int slots;           // rows a block walks at once (one tile)
+    int parts;           // S * tiles: partial results of a sample, blocks of a sample
+    int lgG, lgC;        // log2 of the lanes that reduce one group, one channel
+    int U;               // gcd(V, D): neighbouring channels of a column that are always of one group
+    int tail;            // elements behind the rows
+    bool over_slots;     // lanes of a group's team run over the slots, not over the entries of one
+    unsigned rC, rD, rQT, rUnits;   // gn_div's reciprocals
+    float rM;                // 1 / M
+    float share, share_last; // of a group's values: in a slice, in the last slice with the tail (one tile)
 };
+
+// x / d for x < 2^16, d <= 2^16 with r = ceil(2^32 / d): r d exceeds 2^32 by less than d, so x r / 2^32 exceeds x / d by
+// less than 2^-16 <= 1 / d
+__device__ __forceinline__ int gn_div(int x, unsigned r) { return r ? (int)__umulhi((unsigned)x, r) : x; }   // r == 0: d == 1
 
 // ------------------------------------------------------------------ activations
 template <int A>
@@ -66,286 +88,443 @@ __device__ __forceinline__ void gn_with_act(int act, F&& f) {
     else f(std::integral_constant<int, STMI_ACT_NONE>{});
 }
 
-// ------------------------------------------------------------------ merged statistics
-struct GnPart {
-    float n, mean, m2;
-};
-
-__device__ __forceinline__ GnPart gn_merge(const GnPart& a, const GnPart& b) {
-    const float n = a.n + b.n, r = n > 0.f ? b.n / n : 0.f, d = b.mean - a.mean;
-    if (b.n == 0.f) return a;
-    if (a.n == 0.f) return b;
-    return GnPart{n, a.mean + d * r, a.m2 + b.m2 + d * d * (a.n * r)};
+// ------------------------------------------------------------------ lanes
+template <int kCtrl>
+__device__ __forceinline__ float gn_dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
 }
 
-// lanes of a team (a power of two, within a wave) end with the merge of all of them, in one fixed order
-__device__ __forceinline__ GnPart gn_merge_team(GnPart a, int lanes) {
-    for (int o = 1; o < lanes; o <<= 1) {
-        const GnPart b{__shfl_xor(a.n, o, 64), __shfl_xor(a.mean, o, 64), __shfl_xor(a.m2, o, 64)};
-        a = (threadIdx.x & o) ? gn_merge(b, a) : gn_merge(a, b);
+// the sum of an exchange's two results (the elements are copied first: a bit cast of a vector's element reads element 0)
+__device__ __forceinline__ float gn_add_pair(u32x2 r) {
+    const unsigned lo = r[0], hi = r[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+
+// sum over a team of 2^lg neighbouring lanes, the same bits in every lane of it: partners at distance 1, 2 (within a
+// quad), 4, 8 (mirrored: the lanes of the other half hold equal values), 16, 32 (rows exchanged)
+__device__ __forceinline__ float gn_team_sum(float v, int lg) {
+    if (lg > 0) v += gn_dpp<0xB1>(v);
+    if (lg > 1) v += gn_dpp<0x4E>(v);
+    if (lg > 2) v += gn_dpp<0x141>(v);
+    if (lg > 3) v += gn_dpp<0x140>(v);
+    if (lg > 4) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        v = gn_add_pair(__builtin_amdgcn_permlane16_swap(b, b, false, false));
     }
-    return a;
+    if (lg > 5) {
+        const unsigned b = __builtin_bit_cast(unsigned, v);
+        v = gn_add_pair(__builtin_amdgcn_permlane32_swap(b, b, false, false));
+    }
+    return v;
 }
 
-__device__ __forceinline__ int gn_team_lanes(int teams) {   // power of two
-    int k = 64;
-    while (k > 1 && k * teams > kGnT) k >>= 1;
-    return k;
+// 1 / sqrt(v): the hardware's value (one unit in its last place) and one Newton step
+__device__ __forceinline__ float gn_rsqrt(float v) {
+    const float r = __builtin_amdgcn_rsqf(v);
+    return r + 0.5f * r * (1.f - v * r * r);
 }
 
-// 16 bytes at an element's alignment
-template <typename T, int V>
-__device__ __forceinline__ void gn_load(const T* p, float (&out)[V]) {
-    uint4 raw;
-    __builtin_memcpy(&raw, p, 16);
-    unpack_vec<T, V>(raw, out);
+// ------------------------------------------------------------------ memory
+// 16 bytes at an element's alignment; the address is a block's (scalar) and a thread's offset in bytes; kNt: not kept in
+// the caches
+template <bool kNt>
+__device__ __forceinline__ u32x4 gn_load(const void* p, unsigned own) {
+    typedef u32x4 __attribute__((aligned(2))) loose;
+    const loose* q = reinterpret_cast<const loose*>(static_cast<const char*>(p) + own);
+    if constexpr (kNt) return __builtin_nontemporal_load(q);
+    return *q;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void gn_store(T* p, const float (&in)[V]) {
+template <bool kNt, typename T, int V>
+__device__ __forceinline__ void gn_store(void* p, unsigned own, const float (&in)[V]) {
+    typedef u32x4 __attribute__((aligned(2))) loose;
+    loose* q = reinterpret_cast<loose*>(static_cast<char*>(p) + own);
     T e[V];
 #pragma unroll
     for (int i = 0; i < V; i++) e[i] = from_f32<T>(in[i]);
-    __builtin_memcpy(p, e, 16);
+    u32x4 raw;
+    __builtin_memcpy(&raw, e, 16);
+    if constexpr (kNt) __builtin_nontemporal_store(raw, q);
+    else *q = raw;
 }
 
-// a block's sample, slice and column tile, and what the calling thread owns of the tile
+template <typename T, int V>
+__device__ __forceinline__ void gn_unpack(const u32x4& raw, float (&out)[V]) {
+    T e[V];
+    __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < V; i++) out[i] = to_f32<T>(e[i]);
+}
+
+// ------------------------------------------------------------------ places
+// Blocks run over the parts of a sample first: neighbouring blocks read neighbouring memory.
+constexpr int kGnGridY = 32768;
+__device__ __forceinline__ int gn_sample() { return blockIdx.z * kGnGridY + blockIdx.y; }
+static dim3 gn_grid(int parts, int n) {
+    return dim3((unsigned)parts, (unsigned)(n < kGnGridY ? n : kGnGridY), (unsigned)((n + kGnGridY - 1) / kGnGridY));
+}
+
+// a block's sample, slice and column tile, and what the calling thread owns of the tile.  kTiled: a row has more columns
+// than a block has threads (odd channel counts above 512 only)
+template <bool kTiled>
 struct GnPlace {
-    int n, s, c0, QT, slots, col, slot, r0, r1;
-    bool on;
-    long base, end0;   // the sample's first element; the tail's, behind the rows, within the sample
-    __device__ __forceinline__ explicit GnPlace(const GnGeom& g) {
-        const int per = g.S * g.tiles, t = blockIdx.x % per;
-        n = blockIdx.x / per;
-        s = t / g.tiles;
-        c0 = t % g.tiles * g.QT;
-        QT = min(g.QT, g.Q - c0);
-        slots = kGnT / QT;
-        slot = threadIdx.x / QT;
-        col = c0 + threadIdx.x % QT;
-        on = slot < slots;
-        r0 = min(s * g.rows, g.R);
-        r1 = min(r0 + g.rows, g.R);
-        base = (long)n * g.P * g.C;
-        end0 = (long)g.R * g.L;
+    int n, s, tile, c0, QT, slots, col, slot, rows;
+    long first;        // the slice's first element
+    long end0;         // the tail's first element
+    unsigned own;      // the thread's first element in the slice
+    __device__ __forceinline__ GnPlace(const GnGeom& g, int V) {
+        n = gn_sample();
+        s = blockIdx.x;
+        tile = c0 = 0;
+        QT = g.QT;
+        slots = g.slots;
+        if constexpr (kTiled) {
+            tile = s % g.tiles;
+            s /= g.tiles;
+            c0 = tile * g.QT;
+            QT = min(g.QT, g.Q - c0);
+            slots = kGnT / QT;
+            slot = threadIdx.x / QT;
+        } else {
+            slot = gn_div(threadIdx.x, g.rQT);
+        }
+        col = c0 + threadIdx.x - slot * QT;
+        const int r0 = min(s * g.rows, g.R);
+        rows = min(g.rows, g.R - r0);
+        const long base = (long)n * g.P * g.C;
+        first = base + (long)r0 * g.L;
+        end0 = base + (long)g.R * g.L;
+        own = slot * g.L + col * V;
     }
-    __device__ __forceinline__ bool owns_tail(const GnGeom& g) const { return s == g.S - 1 && c0 == 0; }
+    __device__ __forceinline__ bool on() const { return slot < slots; }
+    __device__ __forceinline__ bool owns_tail(const GnGeom& g) const { return s == g.S - 1 && tile == 0; }
+    __device__ __forceinline__ long part(const GnGeom& g) const { return (long)n * g.parts + blockIdx.x; }
 };
 
+// the entries of a per-channel table in shared memory that belong to a column
+template <int V>
+__device__ __forceinline__ void gn_column(const float* tab, const GnGeom& g, int col, float (&out)[V]) {
+    if (g.L == g.C) {   // whole columns in a pixel: 16-byte reads
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4*>(tab + col * V + j);
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[j + i] = q[i];
+        }
+    } else {
+        int c = col * V - gn_div(col * V, g.rC) * g.C;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            out[j] = tab[c];
+            c = c + 1 == g.C ? 0 : c + 1;
+        }
+    }
+}
+
 // ------------------------------------------------------------------ forward, first launch
-// ws[n][slice * tiles + tile][3][G]: (count, mean, sum of squared deviations) of the block's values of each group.
+// ws[n][slice * tiles + tile][G][2]: (mean, sum of squared deviations) of the block's values of each group; their number
+// follows from the cut (gn_share).
 // A thread keeps a mean and a sum of squared deviations per channel of its column: a batch of kB values is summed as
 // deviations from the mean so far (from the first value in the first batch), then mean += s1 / n, m2 += s2 - s1^2 / n
 // with n the count behind the batch.  That shift is a value of the plane or a mean of some, so s2 exceeds the sum it
 // stands for by no more than the batch's share of the total, and the short batches keep partial sums short.
-template <typename T, int V>
-__global__ __launch_bounds__(kGnT) void gn_stats_kernel(const T* __restrict__ x, float* __restrict__ ws, const GnGeom g) {
+template <typename T, int V, bool kNt, bool kTiled>
+__global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ ws, const GnGeom g) {
     constexpr int kB = 8;
     extern __shared__ float sh[];   // [V][kGnT] means, [V][kGnT] sums of squares, [kGnT] counts
-    const GnPlace p(g);
-    const T* xs = x + p.base;
+    const GnPlace<kTiled> p(g, V);
+    if (p.n >= g.N) return;
     float mean[V], m2[V];
 #pragma unroll
     for (int j = 0; j < V; j++) mean[j] = m2[j] = 0.f;
     int cnt = 0;
-    if (p.on) {
-        const T* xc = xs + (long)p.col * V;
-        for (int row = p.r0 + p.slot; row < p.r1; row += p.slots * kB) {
-            float v[kB][V];
-            int m = 0;
-#pragma unroll
-            for (int u = 0; u < kB; u++) {
-                if (row + u * p.slots < p.r1) {
-                    gn_load<T, V>(xc + (long)(row + u * p.slots) * g.L, v[u]);
-                    m++;
-                }
-            }
-            if (cnt == 0) {
-#pragma unroll
-                for (int j = 0; j < V; j++) mean[j] = v[0][j];
-            }
-            cnt += m;
-            const float rn = 1.f / (float)cnt;
+    if (p.on()) {
+        const T* xb = x + p.first;
+        const unsigned own = p.own * (unsigned)sizeof(T);
+        const int step = p.slots * g.L, batch = kB * p.slots;
+        auto flush = [&](const float (&s1)[V], const float (&s2)[V]) {
+            const float rn = __builtin_amdgcn_rcpf((float)cnt);
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-                for (int u = 0; u < kB; u++) {
-                    const float d = u < m ? v[u][j] - mean[j] : 0.f;
-                    s1 += d;
-                    s2 += d * d;
-                }
-                const float e = s1 * rn;
+                const float e = s1[j] * rn;
                 mean[j] += e;
-                m2[j] += s2 - s1 * e;
+                m2[j] += s2[j] - s1[j] * e;
             }
+        };
+        auto add = [&](const u32x4& raw, float (&s1)[V], float (&s2)[V]) {
+            float v[V];
+            gn_unpack<T, V>(raw, v);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float d = v[j] - mean[j];
+                s1[j] += d;
+                s2[j] += d * d;
+            }
+        };
+        int left = p.rows;
+        for (; left >= batch; left -= batch, xb += kB * (long)step) {
+            u32x4 raw[kB];
+#pragma unroll
+            for (int u = 0; u < kB; u++) raw[u] = gn_load<kNt>(xb + u * (long)step, own);
+            if (cnt == 0) gn_unpack<T, V>(raw[0], mean);
+            float s1[V], s2[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+#pragma unroll
+            for (int u = 0; u < kB; u++) add(raw[u], s1, s2);
+            cnt += kB;
+            flush(s1, s2);
+        }
+        if (p.slot < left) {   // the last, shorter batch
+            u32x4 raw[kB];
+            float s1[V], s2[V];
+#pragma unroll
+            for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+#pragma unroll
+            for (int u = 0; u < kB; u++)
+                if (p.slot < left - u * p.slots) raw[u] = gn_load<kNt>(xb + u * (long)step, own);
+            if (cnt == 0) gn_unpack<T, V>(raw[0], mean);
+#pragma unroll
+            for (int u = 0; u < kB; u++) {
+                if (p.slot < left - u * p.slots) {
+                    add(raw[u], s1, s2);
+                    cnt++;
+                }
+            }
+            flush(s1, s2);
         }
     }
-    // V neighbouring channels of one group are merged in the thread
-    const bool whole = g.D % V == 0;
-    if (whole) {
+    // neighbouring channels of one group are merged in the thread: pairs of equal counts
 #pragma unroll
-        for (int w = 1; w < V; w <<= 1)
+    for (int w = 1; w < V; w <<= 1) {
+        if (w < g.U) {
 #pragma unroll
             for (int j = 0; j < V; j += 2 * w) {
-                const GnPart a = gn_merge(GnPart{(float)(cnt * w), mean[j], m2[j]}, GnPart{(float)(cnt * w), mean[j + w], m2[j + w]});
-                mean[j] = a.mean;
-                m2[j] = a.m2;
+                const float d = mean[j + w] - mean[j];
+                mean[j] += 0.5f * d;
+                m2[j] += m2[j + w] + d * d * (0.5f * (float)(cnt * w));
             }
+        }
     }
     float* lm = sh;
     float* l2 = sh + V * kGnT;
-    int* lc = reinterpret_cast<int*>(sh + 2 * V * kGnT);
+    float* lc = sh + 2 * V * kGnT;
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        if (j && whole) break;
+        if (j & (g.U - 1)) continue;
         lm[j * kGnT + threadIdx.x] = mean[j];
         l2[j * kGnT + threadIdx.x] = m2[j];
     }
-    lc[threadIdx.x] = p.on ? cnt : 0;
+    lc[threadIdx.x] = (float)(cnt * g.U);
     __syncthreads();
-    // a team of lanes merges the entries of one group: `units` per row (channels, or whole columns), every slot
-    const int K = gn_team_lanes(g.G), teams = kGnT / K, lane = threadIdx.x & (K - 1);
-    const int step = whole ? V : 1, reps = g.L / g.C, units = g.D / step, total = units * reps * p.slots;
-    float* out = ws + (((long)p.n * g.S + p.s) * g.tiles + p.c0 / g.QT) * 3 * g.G;
-    for (int gr = threadIdx.x / K; gr < (g.G + teams - 1) / teams * teams; gr += teams) {
-        GnPart a{0.f, 0.f, 0.f};
-        if (gr < g.G) {
-            for (int e = lane; e < total; e += K) {
-                const int slot = e / (units * reps), rest = e - slot * (units * reps), rep = rest / units;
-                const int pos = gr * g.D + (rest - rep * units) * step + rep * g.C;
-                const int col = pos / V - p.c0;
-                if (col < 0 || col >= p.QT) continue;
-                const int t = slot * p.QT + col, j = pos % V;
-                a = gn_merge(a, GnPart{(float)(lc[t] * step), lm[j * kGnT + t], l2[j * kGnT + t]});
-            }
-            if (p.owns_tail(g)) {
-                const int tail = (g.P - (int)(p.end0 / g.C)) * g.D;   // rows are whole pixels
-                for (int e = lane; e < tail; e += K) {
-                    const long at = p.end0 + (long)(e / g.D) * g.C + gr * g.D + e % g.D;
-                    a = gn_merge(a, GnPart{1.f, to_f32<T>(xs[at]), 0.f});
+    // a team of lanes adds the entries of one group up, the means first, then the deviations from their mean
+    const int K = 1 << g.lgG, lane = threadIdx.x & (K - 1);
+    const int units = g.D / g.U, entries = units * (g.L / g.C);
+    const int en0 = g.over_slots ? 0 : lane, enstep = g.over_slots ? 1 : K, sl0 = g.over_slots ? lane : 0, slstep = g.over_slots ? K : 1;
+    float2* out = ws + p.part(g) * g.G;
+    for (int gr0 = 0; gr0 < g.G; gr0 += kGnT >> g.lgG) {
+        const int gr = gr0 + (threadIdx.x >> g.lgG);
+        const bool live = gr < g.G;
+        // f(count, mean, sum of squared deviations) of every entry of the group
+        auto each = [&](auto f) {
+            for (int en = en0; en < entries; en += enstep) {
+                const int rep = gn_div(en, g.rUnits);
+                const int pos = gr * g.D + (en - rep * units) * g.U + rep * g.C, col = pos / V - p.c0, j = pos % V;
+                if (kTiled && (col < 0 || col >= p.QT)) continue;
+                for (int slot = sl0; slot < p.slots; slot += slstep) {
+                    const int t = slot * p.QT + col;
+                    f(lc[t], lm[j * kGnT + t], l2[j * kGnT + t]);
                 }
             }
-        }
-        a = gn_merge_team(a, K);
-        if (gr < g.G && lane == 0) {
-            out[gr] = a.n;
-            out[g.G + gr] = a.mean;
-            out[2 * g.G + gr] = a.m2;
-        }
+            if (g.tail && p.owns_tail(g)) {
+                for (int e = lane; e < g.tail / g.C * g.D; e += K)
+                    f(1.f, to_f32<T>(x[p.end0 + e / g.D * g.C + gr * g.D + e % g.D]), 0.f);
+            }
+        };
+        float n = 0.f, s1 = 0.f, s2 = 0.f;
+        if (live) each([&](float c, float m, float) { n += c; s1 += c * m; });
+        n = gn_team_sum(n, g.lgG);
+        s1 = gn_team_sum(s1, g.lgG);
+        const float mu = n > 0.f ? s1 / n : 0.f;
+        if (live) each([&](float c, float m, float q) { const float d = c > 0.f ? m - mu : 0.f; s2 += q + c * d * d; });
+        s2 = gn_team_sum(s2, g.lgG);
+        if (live && lane == 0) out[gr] = make_float2(mu, s2);
     }
 }
 
-// (mean, 1/sqrt(var + eps)) of group gr of sample n from its partials; every lane of the team ends with them
-__device__ __forceinline__ void gn_fold(const float* __restrict__ ws, const GnGeom& g, int n, int gr, int K, float eps,
+// the share of group gr's values that partial i holds (0 behind the last)
+template <bool kTiled>
+__device__ __forceinline__ float gn_share(const GnGeom& g, int gr, int i) {
+    if constexpr (!kTiled) return i < g.S - 1 ? g.share : i == g.S - 1 ? g.share_last : 0.f;
+    if (i >= g.parts) return 0.f;
+    const int s = i / g.tiles, t = i - s * g.tiles, rows = max(0, min(g.R, (s + 1) * g.rows) - s * g.rows);
+    // positions of the row before e that hold a channel of the group
+    const int V = g.L / g.Q, e0 = t * g.QT * V, e1 = min(g.Q, (t + 1) * g.QT) * V;
+    const int per = e1 / g.C * g.D + min(max(e1 % g.C - gr * g.D, 0), g.D) - e0 / g.C * g.D - min(max(e0 % g.C - gr * g.D, 0), g.D);
+    float n = (float)rows * (float)per;
+    if (s == g.S - 1 && t == 0) n += (float)(g.tail / g.C) * (float)g.D;
+    return n * g.rM;
+}
+
+// (mean, 1/sqrt(var + eps)) of group gr of sample n from its partials, NK at most a lane of the team, in two passes: the
+// mean first, then the deviations from it.  Every lane ends with the result.
+template <int NK, bool kTiled>
+__device__ __forceinline__ void gn_fold_n(const float2* __restrict__ w, const GnGeom& g, int gr, int lg, float eps, float& mean,
+                                          float& rstd) {
+    const int K = 1 << lg, lane = threadIdx.x & (K - 1);
+    float2 r[NK];
+#pragma unroll
+    for (int k = 0; k < NK; k++) r[k] = w[(unsigned)(min(lane + (k << lg), g.parts - 1) * g.G)];
+    float share[NK], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        share[k] = gn_share<kTiled>(g, gr, lane + (k << lg));
+        s1 += share[k] > 0.f ? share[k] * r[k].x : 0.f;
+    }
+    mean = gn_team_sum(s1, lg);
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const float d = r[k].x - mean;
+        s2 += share[k] > 0.f ? r[k].y * g.rM + share[k] * d * d : 0.f;
+    }
+    rstd = gn_rsqrt(gn_team_sum(s2, lg) + eps);
+}
+
+template <bool kTiled>
+__device__ __forceinline__ void gn_fold(const float2* __restrict__ ws, const GnGeom& g, int n, int gr, int lg, float eps,
                                         float& mean, float& rstd) {
-    GnPart a{0.f, 0.f, 0.f};
-    const int parts = g.S * g.tiles;
-    if (gr < g.G) {
-        const float* w = ws + (long)n * parts * 3 * g.G + gr;
-#pragma unroll 4
-        for (int s = threadIdx.x & (K - 1); s < parts; s += K) {
-            const float* r = w + (long)s * 3 * g.G;
-            a = gn_merge(a, GnPart{r[0], r[g.G], r[2 * g.G]});
-        }
-    }
-    a = gn_merge_team(a, K);
-    mean = a.mean;
-    rstd = 1.f / sqrtf(a.m2 / a.n + eps);
+    const float2* w = ws + ((long)n * g.parts * g.G + min(gr, g.G - 1));
+    if (g.parts <= 1 << lg) gn_fold_n<1, kTiled>(w, g, gr, lg, eps, mean, rstd);
+    else if (g.parts <= 2 << lg) gn_fold_n<2, kTiled>(w, g, gr, lg, eps, mean, rstd);
+    else if (g.parts <= 4 << lg) gn_fold_n<4, kTiled>(w, g, gr, lg, eps, mean, rstd);
+    else gn_fold_n<kGnFoldLane, kTiled>(w, g, gr, lg, eps, mean, rstd);
 }
 
-// many partials and groups: folded once by a launch of its own.  grid (N, groups / teams)
-__global__ __launch_bounds__(kGnT) void gn_fold_kernel(const float* __restrict__ ws, float* __restrict__ stats, float eps,
-                                                       const GnGeom g, int K) {
-    const int gr = blockIdx.y * (kGnT / K) + threadIdx.x / K;
+// more partials than the second launch's blocks fold: folded once by a launch of its own.  grid (groups / 8, samples)
+template <bool kTiled>
+__global__ __launch_bounds__(kGnT) void gn_fold_kernel(const float2* __restrict__ ws, float* __restrict__ stats, float eps,
+                                                       const GnGeom g) {
+    const int n = gn_sample(), gr = blockIdx.x * (kGnT / 64) + (threadIdx.x >> 6);
+    if (n >= g.N) return;
     float mean, rstd;
-    gn_fold(ws, g, blockIdx.x, gr, K, eps, mean, rstd);
-    if (gr < g.G && (threadIdx.x & (K - 1)) == 0) {
-        stats[((long)blockIdx.x * g.G + gr) * 2] = mean;
-        stats[((long)blockIdx.x * g.G + gr) * 2 + 1] = rstd;
+    gn_fold<kTiled>(ws, g, n, gr, 6, eps, mean, rstd);
+    if (gr < g.G && (threadIdx.x & 63) == 0) {
+        stats[((long)n * g.G + gr) * 2] = mean;
+        stats[((long)n * g.G + gr) * 2 + 1] = rstd;
     }
-}
-
-// table[2 gr], table[2 gr + 1]: mean and rstd of every group of sample n, in shared memory; ws: folded here (and left in
-// stats by the sample's first block), or NULL: read from stats
-__device__ __forceinline__ void gn_table(float* table, const float* __restrict__ ws, float* __restrict__ stats, float eps,
-                                         const GnGeom& g, int n, bool first) {
-    if (ws) {
-        const int K = gn_team_lanes(g.G), teams = kGnT / K;
-        for (int gr = threadIdx.x / K; gr < (g.G + teams - 1) / teams * teams; gr += teams) {
-            float mean, rstd;
-            gn_fold(ws, g, n, gr, K, eps, mean, rstd);
-            if (gr < g.G && (threadIdx.x & (K - 1)) == 0) {
-                table[2 * gr] = mean;
-                table[2 * gr + 1] = rstd;
-                if (first) {
-                    stats[((long)n * g.G + gr) * 2] = mean;
-                    stats[((long)n * g.G + gr) * 2 + 1] = rstd;
-                }
-            }
-        }
-    } else {
-        for (int i = threadIdx.x; i < 2 * g.G; i += kGnT) table[i] = stats[(long)n * g.G * 2 + i];
-    }
-    __syncthreads();
 }
 
 // ------------------------------------------------------------------ forward, second launch
-// A slice is walked from its end: what the first launch read last is the likeliest to be in a cache still.
-template <typename T, int V>
-__global__ __launch_bounds__(kGnT) void gn_apply_kernel(const T* x, const float* __restrict__ ws, float* __restrict__ stats,
+// ws: the partials, folded here (the sample's first block leaves the statistics), or NULL: statistics come from stats.
+// A slice is walked from its end: what the first launch read last is the likeliest to be in a cache still.  The loads of a
+// thread's first rows are on their way while the block folds the partials and makes its table (mean, scale * rstd, shift of
+// every channel), those of the next rows while it computes.
+template <typename T, int V, bool kNt, bool kRes, bool kTiled>
+__global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const float2* __restrict__ ws, float* __restrict__ stats,
                                                         float eps, const float* __restrict__ scale,
                                                         const float* __restrict__ shift, const T* residual, T* y, int act,
                                                         const GnGeom g) {
     constexpr int kU = 4;
-    extern __shared__ float table[];
-    const GnPlace p(g);
-    gn_table(table, ws, stats, eps, g, p.n, p.s == 0 && p.c0 == 0);
-    const T* xs = x + p.base;
-    const T* rs = residual ? residual + p.base : nullptr;
-    T* ys = y + p.base;
-    gn_with_act(act, [&](auto A) {
-        constexpr int kA = decltype(A)::value;
-        if (p.on) {
-            float mean[V], a[V], b[V];
+    extern __shared__ float tab[];   // [3][C] mean, scale * rstd, shift; [2G]
+    const GnPlace<kTiled> p(g, V);
+    if (p.n >= g.N) return;
+    const int batch = p.slots * kU, full = p.rows / batch, rest = p.rows - full * batch;
+    const int step = p.slots * g.L;
+    const unsigned own = p.own * (unsigned)sizeof(T);
+    const bool on = p.on();
+    long at = p.first + (long)full * kU * step;   // the rest of the rows is walked first, then the batches before it
+    u32x4 raw[kU];
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int c = (p.col * V + j) % g.C, gr = c / g.D;
-                mean[j] = table[2 * gr];
-                a[j] = scale[c] * table[2 * gr + 1];
-                b[j] = shift[c];
-            }
-            const long off = (long)p.col * V;
-            for (int row = p.r1 - 1 - p.slot; row >= p.r0; row -= p.slots * kU) {
-                float v[kU][V], r[kU][V];
+    for (int u = 0; u < kU; u++)
+        if (on && p.slot < rest - u * p.slots) raw[u] = gn_load<kNt>(x + at + u * (long)step, own);
+    u32x4 next[kU];
+    if (on && full > 0) {
 #pragma unroll
-                for (int u = 0; u < kU; u++) {
-                    const int rw = row - u * p.slots;
-                    if (rw < p.r0) continue;
-                    gn_load<T, V>(xs + off + (long)rw * g.L, v[u]);
-                    if (rs) gn_load<T, V>(rs + off + (long)rw * g.L, r[u]);
-                }
-#pragma unroll
-                for (int u = 0; u < kU; u++) {
-                    const int rw = row - u * p.slots;
-                    if (rw < p.r0) continue;
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        v[u][j] = gn_act<kA>((v[u][j] - mean[j]) * a[j] + b[j]);
-                        if (rs) v[u][j] += r[u][j];
-                    }
-                    gn_store<T, V>(ys + off + (long)rw * g.L, v[u]);
+        for (int u = 0; u < kU; u++) next[u] = gn_load<kNt>(x + at - (kU - u) * (long)step, own);
+    }
+    float sc = 0.f, sf = 0.f;
+    if ((int)threadIdx.x < g.C) {
+        sc = scale[threadIdx.x];
+        sf = shift[threadIdx.x];
+    }
+    float* grp = tab + 3 * g.C;
+    if (ws) {
+        for (int gr0 = 0; gr0 < g.G; gr0 += kGnT >> g.lgG) {
+            const int gr = gr0 + (threadIdx.x >> g.lgG);
+            float mean, rstd;
+            gn_fold<kTiled>(ws, g, p.n, gr, g.lgG, eps, mean, rstd);
+            if (gr < g.G && (threadIdx.x & ((1 << g.lgG) - 1)) == 0) {
+                grp[2 * gr] = mean;
+                grp[2 * gr + 1] = rstd;
+                if (blockIdx.x == 0) {
+                    stats[((long)p.n * g.G + gr) * 2] = mean;
+                    stats[((long)p.n * g.G + gr) * 2 + 1] = rstd;
                 }
             }
         }
-        if (p.owns_tail(g)) {
-            const int tail = (int)((long)g.P * g.C - p.end0);
-            for (int e = threadIdx.x; e < tail; e += kGnT) {
-                const long at = p.end0 + e;
-                const int c = e % g.C, gr = c / g.D;
-                float v = gn_act<kA>((to_f32<T>(xs[at]) - table[2 * gr]) * (scale[c] * table[2 * gr + 1]) + shift[c]);
-                if (rs) v += to_f32<T>(rs[at]);
-                ys[at] = from_f32<T>(v);
+    } else {
+        for (int i = threadIdx.x; i < 2 * g.G; i += kGnT) grp[i] = stats[(long)p.n * g.G * 2 + i];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < g.C; c += kGnT) {
+        const int gr = gn_div(c, g.rD);
+        tab[c] = grp[2 * gr];
+        tab[g.C + c] = (c < kGnT ? sc : scale[c]) * grp[2 * gr + 1];
+        tab[2 * g.C + c] = c < kGnT ? sf : shift[c];
+    }
+    __syncthreads();
+    gn_with_act(act, [&](auto A) {
+        constexpr int kA = decltype(A)::value;
+        if (on) {
+            float mean[V], a[V], bb[V];
+            gn_column<V>(tab, g, p.col, mean);
+            gn_column<V>(tab + g.C, g, p.col, a);
+            gn_column<V>(tab + 2 * g.C, g, p.col, bb);
+            auto put = [&](const u32x4& in, const u32x4& res, long where) {
+                float v[V];
+                gn_unpack<T, V>(in, v);
+#pragma unroll
+                for (int j = 0; j < V; j++) v[j] = gn_act<kA>((v[j] - mean[j]) * a[j] + bb[j]);
+                if constexpr (kRes) {
+                    float r[V];
+                    gn_unpack<T, V>(res, r);
+#pragma unroll
+                    for (int j = 0; j < V; j++) v[j] += r[j];
+                }
+                gn_store<kNt, T, V>(y + where, own, v);
+            };
+            u32x4 res[kU];
+            if (p.slot < rest) {
+#pragma unroll
+                for (int u = 0; u < kU; u++) {
+                    if (p.slot < rest - u * p.slots) {
+                        if constexpr (kRes) res[u] = gn_load<kNt>(residual + at + u * (long)step, own);
+                        put(raw[u], res[u], at + u * (long)step);
+                    }
+                }
+            }
+            for (int b = full; b > 0; b--) {
+                at -= kU * (long)step;
+#pragma unroll
+                for (int u = 0; u < kU; u++) {
+                    raw[u] = next[u];
+                    if constexpr (kRes) res[u] = gn_load<kNt>(residual + at + u * (long)step, own);
+                }
+                if (b > 1) {
+#pragma unroll
+                    for (int u = 0; u < kU; u++) next[u] = gn_load<kNt>(x + at - (kU - u) * (long)step, own);
+                }
+#pragma unroll
+                for (int u = 0; u < kU; u++) put(raw[u], res[u], at + u * (long)step);
+            }
+        }
+        if (g.tail && p.owns_tail(g)) {
+            for (int e = threadIdx.x; e < g.tail; e += kGnT) {
+                const long q = p.end0 + e;
+                const int c = e % g.C;
+                float v = gn_act<kA>((to_f32<T>(x[q]) - tab[c]) * tab[g.C + c] + tab[2 * g.C + c]);
+                if constexpr (kRes) v += to_f32<T>(residual[q]);
+                y[q] = from_f32<T>(v);
             }
         }
     });
@@ -353,60 +532,79 @@ __global__ __launch_bounds__(kGnT) void gn_apply_kernel(const T* x, const float*
 
 // ------------------------------------------------------------------ backward, first launch
 // rows[n][slice * tiles + tile][2][C]: the block's sums of g and of g * xhat per channel (the parameter gradients' parts);
-// grows[...][2][G]: the same times scale, per group.  A thread's sums are kept in two levels (kB values, then the rest).
-template <typename T, int V>
-__global__ __launch_bounds__(kGnT) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy,
+// grows[...][G][2]: the same times scale, per group.  (A thread adds few values: 32 of a 1080p plane.)
+template <typename T, int V, bool kNt, bool kTiled>
+__global__ __launch_bounds__(kGnT, 4) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy,
                                                            const float* __restrict__ stats, const float* __restrict__ scale,
                                                            const float* __restrict__ shift, float* __restrict__ rows,
-                                                           float* __restrict__ grows, int act, const GnGeom g) {
+                                                           float2* __restrict__ grows, int act, const GnGeom g) {
     constexpr int kB = 4;
-    extern __shared__ float sh[];   // [V][kGnT] sums of g, [V][kGnT] of g * xhat, [2][C] the block's sums per channel
-    const GnPlace p(g);
-    const T* xs = x + p.base;
-    const T* ds = dy + p.base;
+    extern __shared__ float sh[];   // [3][C] mean, scale * rstd, shift, then [V][kGnT] sums of g, [V][kGnT] of g (x - mean);
+                                    // behind the larger of the two: [2][C] the block's sums per channel
+    const GnPlace<kTiled> p(g, V);
+    if (p.n >= g.N) return;
     const float* st = stats + (long)p.n * g.G * 2;
+    for (int c = threadIdx.x; c < g.C; c += kGnT) {
+        const int gr = gn_div(c, g.rD);
+        sh[c] = st[2 * gr];
+        sh[g.C + c] = scale[c] * st[2 * gr + 1];
+        sh[2 * g.C + c] = shift[c];
+    }
+    __syncthreads();
+    float mean[V], a[V], bb[V];
+    if (p.on()) {
+        gn_column<V>(sh, g, p.col, mean);
+        gn_column<V>(sh + g.C, g, p.col, a);
+        gn_column<V>(sh + 2 * g.C, g, p.col, bb);
+    }
+    __syncthreads();
     float* l1 = sh;
     float* l2 = sh + V * kGnT;
-    float* ch = sh + 2 * V * kGnT;
+    float* ch = sh + max(2 * V * kGnT, 3 * g.C);
+    const unsigned own = p.own * (unsigned)sizeof(T);
+    const int step = p.slots * g.L, batch = kB * p.slots;
     gn_with_act(act, [&](auto A) {
         constexpr int kA = decltype(A)::value;
         float s1[V], s2[V];
 #pragma unroll
         for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
-        if (p.on) {
-            float mean[V], rstd[V], a[V], b[V];
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int c = (p.col * V + j) % g.C, gr = c / g.D;
-                mean[j] = st[2 * gr];
-                rstd[j] = st[2 * gr + 1];
-                a[j] = scale[c] * rstd[j];
-                b[j] = shift[c];
-            }
-            const long off = (long)p.col * V;
-            for (int row = p.r0 + p.slot; row < p.r1; row += p.slots * kB) {
-                float v[kB][V], d[kB][V];
-#pragma unroll
-                for (int u = 0; u < kB; u++) {
-                    const int rw = row + u * p.slots;
-                    if (rw >= p.r1) continue;
-                    gn_load<T, V>(xs + off + (long)rw * g.L, v[u]);
-                    gn_load<T, V>(ds + off + (long)rw * g.L, d[u]);
-                }
+        if (p.on()) {
+            auto add = [&](const u32x4& vr, const u32x4& dr) {
+                float v[V], d[V];
+                gn_unpack<T, V>(vr, v);
+                gn_unpack<T, V>(dr, d);
 #pragma unroll
                 for (int j = 0; j < V; j++) {
-                    float t1 = 0.f, t2 = 0.f;
-#pragma unroll
-                    for (int u = 0; u < kB; u++) {
-                        if (row + u * p.slots >= p.r1) continue;
-                        const float xm = v[u][j] - mean[j];
-                        const float gv = d[u][j] * gn_act_grad<kA>(xm * a[j] + b[j]);
-                        t1 += gv;
-                        t2 += gv * xm;
-                    }
-                    s1[j] += t1;
-                    s2[j] += t2 * rstd[j];
+                    const float xm = v[j] - mean[j];
+                    const float gv = d[j] * gn_act_grad<kA>(xm * a[j] + bb[j]);
+                    s1[j] += gv;
+                    s2[j] += gv * xm;
                 }
+            };
+            const T* xb = x + p.first;
+            const T* db = dy + p.first;
+            int left = p.rows;
+            u32x4 vr[kB], dr[kB];
+            for (; left >= batch; left -= batch, xb += kB * (long)step, db += kB * (long)step) {
+#pragma unroll
+                for (int u = 0; u < kB; u++) {
+                    vr[u] = gn_load<kNt>(xb + u * (long)step, own);
+                    dr[u] = gn_load<kNt>(db + u * (long)step, own);
+                }
+#pragma unroll
+                for (int u = 0; u < kB; u++) add(vr[u], dr[u]);
+            }
+            if (p.slot < left) {   // the last, shorter batch
+#pragma unroll
+                for (int u = 0; u < kB; u++) {
+                    if (p.slot < left - u * p.slots) {
+                        vr[u] = gn_load<kNt>(xb + u * (long)step, own);
+                        dr[u] = gn_load<kNt>(db + u * (long)step, own);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kB; u++)
+                    if (p.slot < left - u * p.slots) add(vr[u], dr[u]);
             }
         }
 #pragma unroll
@@ -416,44 +614,45 @@ __global__ __launch_bounds__(kGnT) void gn_bwd_sums_kernel(const T* __restrict__
         }
         __syncthreads();
         // teams of lanes: one channel each
-        const int K = gn_team_lanes(g.C), teams = kGnT / K, lane = threadIdx.x & (K - 1);
-        const int reps = g.L / g.C, total = reps * p.slots;
-        for (int c = threadIdx.x / K; c < (g.C + teams - 1) / teams * teams; c += teams) {
+        const int K = 1 << g.lgC, lane = threadIdx.x & (K - 1), reps = g.L / g.C;
+        for (int cc = 0; cc < g.C; cc += kGnT >> g.lgC) {
+            const int c = cc + (threadIdx.x >> g.lgC);
+            const bool live = c < g.C;
+            const int gr = gn_div(live ? c : 0, g.rD);
             float t1 = 0.f, t2 = 0.f;
-            if (c < g.C) {
-                for (int e = lane; e < total; e += K) {
-                    const int slot = e / reps, pos = c + (e - slot * reps) * g.C, col = pos / V - p.c0;
-                    if (col < 0 || col >= p.QT) continue;
-                    const int t = slot * p.QT + col, j = pos % V;
-                    t1 += l1[j * kGnT + t];
-                    t2 += l2[j * kGnT + t];
+            if (live) {
+                for (int rep = 0; rep < reps; rep++) {
+                    const int pos = c + rep * g.C, col = pos / V - p.c0, j = pos % V;
+                    if (kTiled && (col < 0 || col >= p.QT)) continue;
+                    for (int slot = lane; slot < p.slots; slot += K) {
+                        t1 += l1[j * kGnT + slot * p.QT + col];
+                        t2 += l2[j * kGnT + slot * p.QT + col];
+                    }
                 }
-                if (p.owns_tail(g)) {
-                    const int pixels = g.P - (int)(p.end0 / g.C), gr = c / g.D;
-                    for (int e = lane; e < pixels; e += K) {
-                        const long at = p.end0 + (long)e * g.C + c;
-                        const float xm = to_f32<T>(xs[at]) - st[2 * gr];
-                        const float gv = to_f32<T>(ds[at]) * gn_act_grad<kA>(xm * (scale[c] * st[2 * gr + 1]) + shift[c]);
+                if (g.tail && p.owns_tail(g)) {
+                    for (int e = lane; e < g.tail / g.C; e += K) {
+                        const long q = p.end0 + e * g.C + c;
+                        const float xm = to_f32<T>(x[q]) - st[2 * gr];
+                        const float gv = to_f32<T>(dy[q]) * gn_act_grad<kA>(xm * (scale[c] * st[2 * gr + 1]) + shift[c]);
                         t1 += gv;
-                        t2 += gv * (xm * st[2 * gr + 1]);
+                        t2 += gv * xm;
                     }
                 }
             }
-            for (int o = 1; o < K; o <<= 1) {
-                t1 += __shfl_xor(t1, o, 64);
-                t2 += __shfl_xor(t2, o, 64);
-            }
-            if (c < g.C && lane == 0) {
+            t1 = gn_team_sum(t1, g.lgC);
+            t2 = gn_team_sum(t2, g.lgC);
+            if (live && lane == 0) {
                 ch[c] = t1;
-                ch[g.C + c] = t2;
+                ch[g.C + c] = t2 * st[2 * gr + 1];
             }
         }
         __syncthreads();
     });
-    const long part = ((long)p.n * g.S + p.s) * g.tiles + p.c0 / g.QT;
+    const long part = p.part(g);
     for (int i = threadIdx.x; i < 2 * g.C; i += kGnT) rows[part * 2 * g.C + i] = ch[i];
-    const int K = gn_team_lanes(g.G), teams = kGnT / K, lane = threadIdx.x & (K - 1);
-    for (int gr = threadIdx.x / K; gr < (g.G + teams - 1) / teams * teams; gr += teams) {
+    const int K = 1 << g.lgG, lane = threadIdx.x & (K - 1);
+    for (int gr0 = 0; gr0 < g.G; gr0 += kGnT >> g.lgG) {
+        const int gr = gr0 + (threadIdx.x >> g.lgG);
         float t1 = 0.f, t2 = 0.f;
         if (gr < g.G) {
             for (int c = gr * g.D + lane; c < (gr + 1) * g.D; c += K) {
@@ -461,58 +660,59 @@ __global__ __launch_bounds__(kGnT) void gn_bwd_sums_kernel(const T* __restrict__
                 t2 += scale[c] * ch[g.C + c];
             }
         }
-        for (int o = 1; o < K; o <<= 1) {
-            t1 += __shfl_xor(t1, o, 64);
-            t2 += __shfl_xor(t2, o, 64);
-        }
-        if (gr < g.G && lane == 0) {
-            grows[part * 2 * g.G + gr] = t1;
-            grows[part * 2 * g.G + g.G + gr] = t2;
-        }
+        t1 = gn_team_sum(t1, g.lgG);
+        t2 = gn_team_sum(t2, g.lgG);
+        if (gr < g.G && lane == 0) grows[part * g.G + gr] = make_float2(t1, t2);
     }
 }
 
-// m[2 gr], m[2 gr + 1] = m1, m2 of group gr of sample n; every lane of the team ends with them
-__device__ __forceinline__ void gn_fold_sums(const float* __restrict__ grows, const GnGeom& g, int n, int gr, int K, float& m1,
-                                             float& m2) {
-    const int parts = g.S * g.tiles;
+// m1, m2 of a group from its partials, as gn_fold
+template <int NK>
+__device__ __forceinline__ void gn_fold_sums_n(const float2* __restrict__ w, const GnGeom& g, int lg, float& m1, float& m2) {
+    const int lane = threadIdx.x & ((1 << lg) - 1);
+    float2 r[NK];
+#pragma unroll
+    for (int k = 0; k < NK; k++) r[k] = w[(unsigned)(min(lane + (k << lg), g.parts - 1) * g.G)];
     m1 = m2 = 0.f;
-    if (gr < g.G) {
-        const float* w = grows + (long)n * parts * 2 * g.G + gr;
-#pragma unroll 4
-        for (int s = threadIdx.x & (K - 1); s < parts; s += K) {
-            m1 += w[(long)s * 2 * g.G];
-            m2 += w[(long)s * 2 * g.G + g.G];
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        if (lane + (k << lg) < g.parts) {
+            m1 += r[k].x;
+            m2 += r[k].y;
         }
     }
-    for (int o = 1; o < K; o <<= 1) {
-        m1 += __shfl_xor(m1, o, 64);
-        m2 += __shfl_xor(m2, o, 64);
-    }
-    const float M = (float)g.P * (float)g.D;
-    m1 /= M;
-    m2 /= M;
+    m1 = gn_team_sum(m1, lg) * g.rM;
+    m2 = gn_team_sum(m2, lg) * g.rM;
 }
 
-__global__ __launch_bounds__(kGnT) void gn_fold_sums_kernel(const float* __restrict__ grows, float* __restrict__ m,
-                                                            const GnGeom g, int K) {
-    const int gr = blockIdx.y * (kGnT / K) + threadIdx.x / K;
+__device__ __forceinline__ void gn_fold_sums(const float2* __restrict__ grows, const GnGeom& g, int n, int gr, int lg, float& m1,
+                                             float& m2) {
+    const float2* w = grows + ((long)n * g.parts * g.G + min(gr, g.G - 1));
+    if (g.parts <= 1 << lg) gn_fold_sums_n<1>(w, g, lg, m1, m2);
+    else if (g.parts <= 2 << lg) gn_fold_sums_n<2>(w, g, lg, m1, m2);
+    else if (g.parts <= 4 << lg) gn_fold_sums_n<4>(w, g, lg, m1, m2);
+    else gn_fold_sums_n<kGnFoldLane>(w, g, lg, m1, m2);
+}
+
+__global__ __launch_bounds__(kGnT) void gn_fold_sums_kernel(const float2* __restrict__ grows, float* __restrict__ m, const GnGeom g) {
+    const int n = gn_sample(), gr = blockIdx.x * (kGnT / 64) + (threadIdx.x >> 6);
+    if (n >= g.N) return;
     float m1, m2;
-    gn_fold_sums(grows, g, blockIdx.x, gr, K, m1, m2);
-    if (gr < g.G && (threadIdx.x & (K - 1)) == 0) {
-        m[((long)blockIdx.x * g.G + gr) * 2] = m1;
-        m[((long)blockIdx.x * g.G + gr) * 2 + 1] = m2;
+    gn_fold_sums(grows, g, n, gr, 6, m1, m2);
+    if (gr < g.G && (threadIdx.x & 63) == 0) {
+        m[((long)n * g.G + gr) * 2] = m1;
+        m[((long)n * g.G + gr) * 2 + 1] = m2;
     }
 }
 
 // dshift / dscale from the partial rows: outputs o of [0, 2C), 64 a block, eight row groups each, in one fixed order
-__device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, int nrows, float* __restrict__ dscale,
+__device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, long nrows, float* __restrict__ dscale,
                                                float* __restrict__ dshift, int accumulate, int C, int block, float* tmp) {
     const int o = block * 64 + (threadIdx.x & 63), rg = threadIdx.x >> 6;
     float s = 0.f;
     if (o < 2 * C) {
 #pragma unroll 8
-        for (int i = rg; i < nrows; i += kGnT / 64) s += rows[(long)i * 2 * C + o];
+        for (long i = rg; i < nrows; i += kGnT / 64) s += rows[i * 2 * C + o];
     }
     tmp[threadIdx.x] = s;
     __syncthreads();
@@ -525,88 +725,370 @@ __device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, i
 }
 
 // ------------------------------------------------------------------ backward, second launch
-// The last blocks fold the parameter gradients, the others write dx.
-template <typename T, int V>
-__global__ __launch_bounds__(kGnT) void gn_bwd_apply_kernel(const T* x, const T* dy, const float* __restrict__ stats,
+// The last blocks fold the parameter gradients, the others write dx.  As in the forward pass a slice is walked from its
+// end, and loads are on their way during the fold and the computation of the rows before.
+template <typename T, int V, bool kNt, bool kTiled>
+__global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const T* dy, const float* __restrict__ stats,
                                                             const float* __restrict__ scale, const float* __restrict__ shift,
-                                                            const float* __restrict__ grows, const float* __restrict__ msums,
+                                                            const float2* __restrict__ grows, const float* __restrict__ msums,
                                                             const float* __restrict__ rows, T* dx, float* dscale, float* dshift,
                                                             int accumulate, int act, const GnGeom g) {
     constexpr int kU = 2;
-    extern __shared__ float table[];   // [2G] m1, m2 (512 floats at least)
-    const int main_blocks = g.N * g.S * g.tiles;
-    if ((int)blockIdx.x >= main_blocks) {
-        gn_param_grads(rows, main_blocks, dscale, dshift, accumulate, g.C, blockIdx.x - main_blocks, table);
+    // [5][C] mean, scale * rstd, shift, k1 = rstd m1, k2 = rstd^2 m2 with dx = scale rstd g - k1 - (x - mean) k2; [2G] m1, m2
+    // (512 floats at least)
+    extern __shared__ float tab[];
+    if ((int)blockIdx.x >= g.parts) {
+        const long q = (long)(blockIdx.x - g.parts) * g.N + gn_sample();
+        if (gn_sample() < g.N && q * 64 < 2 * g.C) gn_param_grads(rows, (long)g.N * g.parts, dscale, dshift, accumulate, g.C, (int)q, tab);
         return;
     }
-    const GnPlace p(g);
-    const T* xs = x + p.base;
-    const T* ds = dy + p.base;
-    T* os = dx + p.base;
+    const GnPlace<kTiled> p(g, V);
+    if (p.n >= g.N) return;
+    const int batch = p.slots * kU, full = p.rows / batch, rest = p.rows - full * batch;
+    const int step = p.slots * g.L;
+    const unsigned own = p.own * (unsigned)sizeof(T);
+    const bool on = p.on();
+    long at = p.first + (long)full * kU * step;
+    u32x4 vr[kU], dr[kU], vn[kU], dn[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+        if (on && p.slot < rest - u * p.slots) {
+            vr[u] = gn_load<kNt>(x + at + u * (long)step, own);
+            dr[u] = gn_load<kNt>(dy + at + u * (long)step, own);
+        }
+    }
+    if (on && full > 0) {
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            vn[u] = gn_load<kNt>(x + at - (kU - u) * (long)step, own);
+            dn[u] = gn_load<kNt>(dy + at - (kU - u) * (long)step, own);
+        }
+    }
     const float* st = stats + (long)p.n * g.G * 2;
+    float* grp = tab + 5 * g.C;
     if (msums) {
-        for (int i = threadIdx.x; i < 2 * g.G; i += kGnT) table[i] = msums[(long)p.n * g.G * 2 + i];
+        for (int i = threadIdx.x; i < 2 * g.G; i += kGnT) grp[i] = msums[(long)p.n * g.G * 2 + i];
     } else {
-        const int K = gn_team_lanes(g.G), teams = kGnT / K;
-        for (int gr = threadIdx.x / K; gr < (g.G + teams - 1) / teams * teams; gr += teams) {
+        for (int gr0 = 0; gr0 < g.G; gr0 += kGnT >> g.lgG) {
+            const int gr = gr0 + (threadIdx.x >> g.lgG);
             float m1, m2;
-            gn_fold_sums(grows, g, p.n, gr, K, m1, m2);
-            if (gr < g.G && (threadIdx.x & (K - 1)) == 0) {
-                table[2 * gr] = m1;
-                table[2 * gr + 1] = m2;
+            gn_fold_sums(grows, g, p.n, gr, g.lgG, m1, m2);
+            if (gr < g.G && (threadIdx.x & ((1 << g.lgG) - 1)) == 0) {
+                grp[2 * gr] = m1;
+                grp[2 * gr + 1] = m2;
             }
         }
     }
     __syncthreads();
+    for (int c = threadIdx.x; c < g.C; c += kGnT) {
+        const int gr = gn_div(c, g.rD);
+        const float rstd = st[2 * gr + 1];
+        tab[c] = st[2 * gr];
+        tab[g.C + c] = scale[c] * rstd;
+        tab[2 * g.C + c] = shift[c];
+        tab[3 * g.C + c] = rstd * grp[2 * gr];
+        tab[4 * g.C + c] = rstd * rstd * grp[2 * gr + 1];
+    }
+    __syncthreads();
     gn_with_act(act, [&](auto A) {
         constexpr int kA = decltype(A)::value;
-        if (p.on) {
-            // dx = a g - k1 - (x - mean) k2 with a = scale rstd, k1 = rstd m1, k2 = rstd^2 m2
-            float mean[V], a[V], b[V], k1[V], k2[V];
+        if (on) {
+            float mean[V], a[V], bb[V], k1[V], k2[V];
+            gn_column<V>(tab, g, p.col, mean);
+            gn_column<V>(tab + g.C, g, p.col, a);
+            gn_column<V>(tab + 2 * g.C, g, p.col, bb);
+            gn_column<V>(tab + 3 * g.C, g, p.col, k1);
+            gn_column<V>(tab + 4 * g.C, g, p.col, k2);
+            auto put = [&](const u32x4& vi, const u32x4& di, long where) {
+                float v[V], d[V];
+                gn_unpack<T, V>(vi, v);
+                gn_unpack<T, V>(di, d);
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int c = (p.col * V + j) % g.C, gr = c / g.D;
-                const float rstd = st[2 * gr + 1];
-                mean[j] = st[2 * gr];
-                a[j] = scale[c] * rstd;
-                b[j] = shift[c];
-                k1[j] = rstd * table[2 * gr];
-                k2[j] = rstd * rstd * table[2 * gr + 1];
+                for (int j = 0; j < V; j++) {
+                    const float xm = v[j] - mean[j];
+                    v[j] = d[j] * gn_act_grad<kA>(xm * a[j] + bb[j]) * a[j] - k1[j] - xm * k2[j];
+                }
+                gn_store<kNt, T, V>(dx + where, own, v);
+            };
+            if (p.slot < rest) {
+#pragma unroll
+                for (int u = 0; u < kU; u++)
+                    if (p.slot < rest - u * p.slots) put(vr[u], dr[u], at + u * (long)step);
             }
-            const long off = (long)p.col * V;
-            for (int row = p.r1 - 1 - p.slot; row >= p.r0; row -= p.slots * kU) {
-                float v[kU][V], d[kU][V];
+            for (int b = full; b > 0; b--) {
+                at -= kU * (long)step;
 #pragma unroll
                 for (int u = 0; u < kU; u++) {
-                    const int rw = row - u * p.slots;
-                    if (rw < p.r0) continue;
-                    gn_load<T, V>(xs + off + (long)rw * g.L, v[u]);
-                    gn_load<T, V>(ds + off + (long)rw * g.L, d[u]);
+                    vr[u] = vn[u];
+                    dr[u] = dn[u];
                 }
+                if (b > 1) {
 #pragma unroll
-                for (int u = 0; u < kU; u++) {
-                    const int rw = row - u * p.slots;
-                    if (rw < p.r0) continue;
-#pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        const float xm = v[u][j] - mean[j];
-                        v[u][j] = d[u][j] * gn_act_grad<kA>(xm * a[j] + b[j]) * a[j] - k1[j] - xm * k2[j];
+                    for (int u = 0; u < kU; u++) {
+                        vn[u] = gn_load<kNt>(x + at - (kU - u) * (long)step, own);
+                        dn[u] = gn_load<kNt>(dy + at - (kU - u) * (long)step, own);
                     }
-                    gn_store<T, V>(os + off + (long)rw * g.L, v[u]);
                 }
+#pragma unroll
+                for (int u = 0; u < kU; u++) put(vr[u], dr[u], at + u * (long)step);
             }
         }
-        if (p.owns_tail(g)) {
-            const int tail = (int)((long)g.P * g.C - p.end0);
-            for (int e = threadIdx.x; e < tail; e += kGnT) {
-                const long at = p.end0 + e;
-                const int c = e % g.C, gr = c / g.D;
-                const float rstd = st[2 * gr + 1], a = scale[c] * rstd, xm = to_f32<T>(xs[at]) - st[2 * gr];
-                os[at] = from_f32<T>(to_f32<T>(ds[at]) * gn_act_grad<kA>(xm * a + shift[c]) * a - rstd * table[2 * gr] -
-                                     xm * (rstd * rstd * table[2 * gr + 1]));
+        if (g.tail && p.owns_tail(g)) {
+            for (int e = threadIdx.x; e < g.tail; e += kGnT) {
+                const long q = p.end0 + e;
+                const int c = e % g.C;
+                const float xm = to_f32<T>(x[q]) - tab[c], sa = tab[g.C + c];
+                dx[q] = from_f32<T>(to_f32<T>(dy[q]) * gn_act_grad<kA>(xm * sa + tab[2 * g.C + c]) * sa - tab[3 * g.C + c] -
+                                    xm * tab[4 * g.C + c]);
             }
         }
     });
+}
+
+// ------------------------------------------------------------------ small samples: one launch
+// A unit is one group, or the V / D groups of one 16-byte column where D < V; its P pixels x DV columns stay in the
+// registers of ONE block: read once, the mean first, then the deviations from it, then the result.  Neighbouring units
+// share cache lines: the block numbers are dealt so that they run on one XCD (one L2).
+struct GnUnit {
+    int n, unit, DV, Ta, col, pix, dpix;
+    long at;   // the thread's first vector, in elements
+    __device__ __forceinline__ GnUnit(const GnGeom& g, int V) {
+        const unsigned w = max(g.D, V), units = g.C / w, lin = (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
+        n = lin / units;
+        unit = lin - n * units;
+        DV = w / V;
+        dpix = blockDim.x / DV;
+        Ta = dpix * DV;
+        pix = gn_div(threadIdx.x, g.rQT);   // the launcher's: of DV
+        col = threadIdx.x - pix * DV;
+        if ((int)threadIdx.x >= Ta) pix = g.P;
+        at = ((long)n * g.P + pix) * g.C + (long)unit * w + col * V;
+    }
+};
+
+// sums of NS values over the block, in every thread; red: [16][NS]
+template <int NS>
+__device__ __forceinline__ void gn_block_sums(float (&v)[NS], float* red) {
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+#pragma unroll
+    for (int k = 0; k < NS; k++) v[k] = gn_team_sum(v[k], 6);
+    if (waves == 1) return;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int k = 0; k < NS; k++) red[wave * NS + k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NS; k++) v[k] = 0.f;
+    for (int w = 0; w < waves; w++)
+#pragma unroll
+        for (int k = 0; k < NS; k++) v[k] += red[w * NS + k];
+}
+
+template <typename T, int V, int NS, int kU>
+__global__ __launch_bounds__(1024) void gn_unit_fwd_kernel(const T* x, float* __restrict__ stats, float eps,
+                                                           const float* __restrict__ scale, const float* __restrict__ shift,
+                                                           const T* residual, T* y, int act, const GnGeom g) {
+    constexpr int W = V / NS;   // channels of a column that share a group
+    __shared__ float red[16 * NS];
+    const GnUnit u_(g, V);
+    if (u_.n >= g.N) return;
+    const long step = (long)u_.dpix * g.C;
+    u32x4 raw[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++)
+        if (u_.pix + u * u_.dpix < g.P) raw[u] = gn_load<false>(x + u_.at + u * step, 0);
+    const int c0 = u_.unit * max(g.D, V) + u_.col * V;
+    float a[V], b[V];
+    if (u_.pix < g.P) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            a[j] = scale[c0 + j];
+            b[j] = shift[c0 + j];
+        }
+    }
+    const float rM = g.rM;
+    float mean[NS], rstd[NS];
+#pragma unroll
+    for (int k = 0; k < NS; k++) mean[k] = rstd[k] = 0.f;
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+        if (u_.pix + u * u_.dpix < g.P) {
+            float v[V];
+            gn_unpack<T, V>(raw[u], v);
+#pragma unroll
+            for (int j = 0; j < V; j++) mean[j / W] += v[j];
+        }
+    }
+    gn_block_sums<NS>(mean, red);
+#pragma unroll
+    for (int k = 0; k < NS; k++) mean[k] *= rM;
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+        if (u_.pix + u * u_.dpix < g.P) {
+            float v[V];
+            gn_unpack<T, V>(raw[u], v);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float d = v[j] - mean[j / W];
+                rstd[j / W] += d * d;
+            }
+        }
+    }
+    gn_block_sums<NS>(rstd, red);
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        rstd[k] = gn_rsqrt(rstd[k] * rM + eps);
+        if (threadIdx.x == 0) {
+            float* st = stats + ((long)u_.n * g.G + u_.unit * NS + k) * 2;
+            st[0] = mean[k];
+            st[1] = rstd[k];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) a[j] *= rstd[j / W];
+    gn_with_act(act, [&](auto A) {
+        constexpr int kA = decltype(A)::value;
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            if (u_.pix + u * u_.dpix < g.P) {
+                float v[V];
+                gn_unpack<T, V>(raw[u], v);
+#pragma unroll
+                for (int j = 0; j < V; j++) v[j] = gn_act<kA>((v[j] - mean[j / W]) * a[j] + b[j]);
+                if (residual) {
+                    float r[V];
+                    gn_unpack<T, V>(gn_load<false>(residual + u_.at + u * step, 0), r);
+#pragma unroll
+                    for (int j = 0; j < V; j++) v[j] += r[j];
+                }
+                gn_store<false, T, V>(y + u_.at + u * step, 0, v);
+            }
+        }
+    });
+}
+
+// rows[n][2][C]: the sample's sums of g and g * xhat per channel; for one sample the parameter gradients themselves
+template <typename T, int V, int NS, int kU>
+__global__ __launch_bounds__(512) void gn_unit_bwd_kernel(const T* x, const T* dy, const float* __restrict__ stats,
+                                                          const float* __restrict__ scale, const float* __restrict__ shift,
+                                                          T* dx, float* __restrict__ rows, float* dscale, float* dshift,
+                                                          int accumulate, int act, const GnGeom g) {
+    constexpr int W = V / NS;
+    extern __shared__ float sh[];   // [2][V][blockDim] the threads' sums
+    __shared__ float red[8 * 2 * NS];
+    const GnUnit u_(g, V);
+    if (u_.n >= g.N) return;
+    const int T_ = blockDim.x, wide = max(g.D, V), c0 = u_.unit * wide;
+    const long step = (long)u_.dpix * g.C;
+    u32x4 vr[kU], dr[kU];
+#pragma unroll
+    for (int u = 0; u < kU; u++) {
+        if (u_.pix + u * u_.dpix < g.P) {
+            vr[u] = gn_load<false>(x + u_.at + u * step, 0);
+            dr[u] = gn_load<false>(dy + u_.at + u * step, 0);
+        }
+    }
+    float a[V], b[V], mean[NS], rstd[NS];
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        const float* st = stats + ((long)u_.n * g.G + u_.unit * NS + k) * 2;
+        mean[k] = st[0];
+        rstd[k] = st[1];
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        a[j] = scale[c0 + u_.col * V + j] * rstd[j / W];
+        b[j] = shift[c0 + u_.col * V + j];
+    }
+    gn_with_act(act, [&](auto A) {
+        constexpr int kA = decltype(A)::value;
+        float s1[V], s2[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) s1[j] = s2[j] = 0.f;
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            if (u_.pix + u * u_.dpix < g.P) {
+                float v[V], d[V];
+                gn_unpack<T, V>(vr[u], v);
+                gn_unpack<T, V>(dr[u], d);
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float xm = v[j] - mean[j / W];
+                    const float gv = d[j] * gn_act_grad<kA>(xm * a[j] + b[j]);
+                    s1[j] += gv;
+                    s2[j] += gv * xm;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            sh[j * T_ + threadIdx.x] = s1[j];
+            sh[(V + j) * T_ + threadIdx.x] = s2[j] * rstd[j / W];
+        }
+        // m1, m2: scale times the sums over the unit's channels, straight from the threads' sums
+        float m[2 * NS];
+#pragma unroll
+        for (int k = 0; k < 2 * NS; k++) m[k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            m[j / W] += a[j] * s1[j];            // rstd times the wanted sum
+            m[NS + j / W] += a[j] * s2[j];       // the wanted sum: the product with rstd makes xhat
+        }
+        gn_block_sums<2 * NS>(m, red);
+        const float rM = g.rM;
+        // dx = a g - k1 - (x - mean) k2,  k1 = rstd m1,  k2 = rstd^2 m2
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            m[k] *= rM;
+            m[NS + k] *= rM * rstd[k] * rstd[k];
+        }
+#pragma unroll
+        for (int u = 0; u < kU; u++) {
+            if (u_.pix + u * u_.dpix < g.P) {
+                float v[V], d[V];
+                gn_unpack<T, V>(vr[u], v);
+                gn_unpack<T, V>(dr[u], d);
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float xm = v[j] - mean[j / W];
+                    v[j] = d[j] * gn_act_grad<kA>(xm * a[j] + b[j]) * a[j] - m[j / W] - xm * m[NS + j / W];
+                }
+                gn_store<false, T, V>(dx + u_.at + u * step, 0, v);
+            }
+        }
+    });
+    if (!rows && !dscale) return;
+    __syncthreads();
+    // per channel: a team of lanes adds the slots' sums
+    const int K = 1 << g.lgC, lane = threadIdx.x & (K - 1), teams = T_ >> g.lgC;   // lgC: the launcher's, of max(D, V)
+    for (int cc = 0; cc < wide; cc += teams) {
+        const int c = cc + (threadIdx.x >> g.lgC);
+        float t1 = 0.f, t2 = 0.f;
+        if (c < wide) {
+            for (int slot = lane; slot < u_.dpix; slot += K) {
+                t1 += sh[(c % V) * T_ + slot * u_.DV + c / V];
+                t2 += sh[(V + c % V) * T_ + slot * u_.DV + c / V];
+            }
+        }
+        t1 = gn_team_sum(t1, g.lgC);
+        t2 = gn_team_sum(t2, g.lgC);
+        if (c < wide && lane == 0) {
+            if (rows) {
+                rows[((long)u_.n * 2) * g.C + c0 + c] = t1;
+                rows[((long)u_.n * 2 + 1) * g.C + c0 + c] = t2;
+            } else {
+                dshift[c0 + c] = accumulate ? dshift[c0 + c] + t1 : t1;
+                dscale[c0 + c] = accumulate ? dscale[c0 + c] + t2 : t2;
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(kGnT) void gn_param_grads_kernel(const float* __restrict__ rows, long nrows, float* dscale,
+                                                              float* dshift, int accumulate, int C) {
+    __shared__ float tmp[kGnT];
+    gn_param_grads(rows, nrows, dscale, dshift, accumulate, C, blockIdx.x, tmp);
 }
 
 __global__ __launch_bounds__(256) void gn_zero_kernel(float* a, float* b, int n) {
@@ -615,6 +1097,15 @@ __global__ __launch_bounds__(256) void gn_zero_kernel(float* a, float* b, int n)
 }
 
 // ------------------------------------------------------------------ launches
+// log2 of the lanes (64 at most) that `teams` teams of a block of `threads` have each
+static int gn_lg_lanes(int teams, int threads) {
+    int lg = 6;
+    while (lg > 0 && (teams << lg) > threads) lg--;
+    return lg;
+}
+
+static unsigned gn_recip(int d) { return d == 1 ? 0u : (unsigned)(((1UL << 32) + d - 1) / d); }
+
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
 static GnGeom gn_geom(int n, int P, int c, int groups, int V) {
@@ -622,47 +1113,136 @@ static GnGeom gn_geom(int n, int P, int c, int groups, int V) {
     g.N = n; g.P = P; g.C = c; g.G = groups; g.D = c / groups;
     g.L = c / gcd_int(c, V) * V;
     g.Q = g.L / V;
+    g.U = gcd_int(V, g.D);
     g.QT = g.Q < kGnT ? g.Q : kGnT;
     g.tiles = ceil_div(g.Q, g.QT);
-    const int slots = kGnT / g.QT;
+    g.slots = kGnT / g.QT;
     g.R = (int)((long)P * c / g.L);
-    // four rows a thread at least; a sample is cut the same way whatever its batch
-    int S = ceil_div(kGnSlices, g.tiles);
-    if (S > g.R / (slots * 4)) S = g.R / (slots * 4);
+    g.tail = (int)((long)P * c - (long)g.R * g.L);
+    g.lgG = gn_lg_lanes(groups, kGnT);
+    g.lgC = gn_lg_lanes(c, kGnT);
+    // A sample is cut the same way whatever its batch: slices of four rows a thread (32 KB) for the smaller samples, up to
+    // kGnSlices larger ones for the larger.
+    const int per4 = g.R / (g.slots * 4);
+    int S = per4 < 128 ? per4 : per4 < 256 ? 128 : per4 / 2;
+    // few enough partials for the second launch to fold, unless the sample is large (32 MB) or would be cut in too few
+    const int few = (kGnFoldLane << g.lgG) / g.tiles;
+    if (S > few && few >= 64 && (long)P * c / V * 16 <= (32L << 20)) S = few;
+    if (S > kGnSlices / g.tiles) S = kGnSlices / g.tiles;
     if (S < 1) S = 1;
     g.rows = ceil_div(g.R, S);
     if (g.rows < 1) g.rows = 1;
     g.S = ceil_div(g.R, g.rows);
     if (g.S < 1) g.S = 1;
+    g.parts = g.S * g.tiles;
+    const int units = g.D / g.U, entries = units * (g.L / c), K = 1 << g.lgG;
+    g.over_slots = entries * ceil_div(g.slots, K) <= g.slots * ceil_div(entries, K);
+    g.rC = gn_recip(c);
+    g.rD = gn_recip(g.D);
+    g.rQT = gn_recip(g.QT);
+    g.rUnits = gn_recip(units);
+    const double M = (double)P * g.D, pixels = (double)g.L / c;
+    const int last = g.R - (g.S - 1) * g.rows;
+    g.rM = (float)(1.0 / M);
+    g.share = (float)(g.rows * pixels * g.D / M);
+    g.share_last = (float)((last * pixels + g.tail / c) * g.D / M);
     return g;
 }
 
-static bool gn_folds_itself(const GnGeom& g) { return (long)g.S * g.tiles * g.G <= kGnFold; }
+// the second launch's blocks fold the partials themselves
+static bool gn_folds_itself(const GnGeom& g) { return g.parts <= kGnFoldLane << g.lgG; }
 
-// enough for either direction
-long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype) {
-    const GnGeom g = gn_geom(n, h * w, c, groups, dtype == STMI_BF16 ? 8 : 4);
-    const long parts = (long)n * g.S * g.tiles;
-    return parts * 2 * c + parts * 3 * groups + (long)n * 2 * groups;
+// One block per unit, if a unit's vectors fit its registers: threads and vectors a thread, or false.
+// STMI_NO_GN_UNITS: never (tests compare the two forms).
+static bool gn_in_units(const GnGeom& g, int V, int most_threads, int* threads, int* u) {
+    if (g.C % V || (g.D % V && V % g.D) || STMI_ENV_SET("STMI_NO_GN_UNITS")) return false;
+    const int DV = (g.D > V ? g.D : V) / V;
+    const long nv = (long)g.P * DV;
+    // A unit 16 bytes wide reads every cache line in pieces.  Graph of 20 calls, us, one block per unit / slices: 2025 pixels
+    // 16 bytes wide 6.0 / 8.8 forward and 8.5 / 12.2 backward (one sample of 64 channels), 4096 pixels 8.9 / 8.7 and 13.1 / 11.5;
+    // 32 bytes wide, 4096 pixels 12.2 / 11.2 (one sample of 512 channels), 33.7 / 51.8 (16 samples), 64 bytes 22.1 / 47.2.
+    if (DV == 1 && nv > 2048) return false;
+    for (*u = 2; *u <= 8; *u *= 2)
+        for (*threads = 64; *threads <= most_threads; *threads *= 2)
+            if ((long)(*threads / DV * DV) * *u >= nv) return true;
+    return false;
+}
+
+long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward) {
+    const int V = dtype == STMI_BF16 ? 8 : 4;
+    const GnGeom g = gn_geom(n, h * w, c, groups, V);
+    const long parts = (long)n * g.parts;
+    int threads, u;
+    if (gn_in_units(g, V, backward ? kGnUnitBwd : kGnUnitFwd, &threads, &u)) return backward && n > 1 ? (long)n * 2 * c : 0;
+    return backward ? parts * 2 * c + parts * 2 * groups + (long)n * 2 * groups : parts * 2 * groups;
+}
+
+// f(groups of a column, vectors of a thread) as compile-time constants
+template <int V, typename F>
+static void gn_unit_launch(const GnGeom& g, int u, F&& f) {
+    auto with_u = [&](auto NS) {
+        if (u == 2) f(NS, std::integral_constant<int, 2>{});
+        else if (u == 4) f(NS, std::integral_constant<int, 4>{});
+        else f(NS, std::integral_constant<int, 8>{});
+    };
+    const int ns = g.D >= V ? 1 : V / g.D;
+    if (ns == 1) with_u(std::integral_constant<int, 1>{});
+    else if (ns == 2) with_u(std::integral_constant<int, 2>{});
+    else if (ns == 4) with_u(std::integral_constant<int, 4>{});
+    else with_u(std::integral_constant<int, V>{});
+}
+
+// Tensors that together exceed the last-level cache (256 MB) are streamed past it.
+static bool gn_streams(int tensors, int n, int P, int c, int size) { return (long)tensors * n * P * c * size > (256L << 20); }
+
+// f(kNt, kTiled) as compile-time constants; rows of several tiles are rare (odd channel counts above 512): one form
+template <typename F>
+static int gn_with_form(bool nt, const GnGeom& g, F&& f) {
+    if (g.tiles > 1) return f(std::false_type{}, std::true_type{});
+    if (nt) return f(std::true_type{}, std::false_type{});
+    return f(std::false_type{}, std::false_type{});
 }
 
 template <typename T, int V>
 static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float* scale, const float* shift, const T* residual,
                     T* y, int act, int n, int P, int c, int groups, hipStream_t s) {
-    const GnGeom g = gn_geom(n, P, c, groups, V);
-    const dim3 grid((unsigned)(g.N * g.S * g.tiles));
-    hipLaunchKernelGGL((gn_stats_kernel<T, V>), grid, dim3(kGnT), (2 * V + 1) * kGnT * sizeof(float), s, x, ws, g);
-    STMI_LAUNCH_CHECK("gn_stats_kernel");
-    const float* fold = ws;
-    if (!gn_folds_itself(g)) {
-        hipLaunchKernelGGL(gn_fold_kernel, dim3(g.N, ceil_div(g.G, kGnT / 64)), dim3(kGnT), 0, s, (const float*)ws, stats, eps, g, 64);
-        STMI_LAUNCH_CHECK("gn_fold_kernel");
-        fold = nullptr;
+    GnGeom g = gn_geom(n, P, c, groups, V);
+    int threads, u;
+    if (gn_in_units(g, V, kGnUnitFwd, &threads, &u)) {
+        const int wide = g.D > V ? g.D : V;
+        const dim3 grid((unsigned)ceil_div((long)n * (c / wide), 8) * 8);
+        g.rQT = gn_recip(wide / V);
+        gn_unit_launch<V>(g, u, [&](auto NS, auto U) {
+            hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads), 0, s, x, stats,
+                               eps, scale, shift, residual, y, act, g);
+        });
+        STMI_LAUNCH_CHECK("gn_unit_fwd_kernel");
+        return STMI_OK;
     }
-    hipLaunchKernelGGL((gn_apply_kernel<T, V>), grid, dim3(kGnT), 2 * g.G * sizeof(float), s, x, fold, stats, eps, scale, shift,
-                       residual, y, act, g);
-    STMI_LAUNCH_CHECK("gn_apply_kernel");
-    return STMI_OK;
+    return gn_with_form(gn_streams(residual ? 3 : 2, n, P, c, sizeof(T)), g, [&](auto NT, auto TL) -> int {
+        constexpr bool kNt = decltype(NT)::value, kTiled = decltype(TL)::value;
+        const dim3 grid = gn_grid(g.parts, n);
+        hipLaunchKernelGGL((gn_stats_kernel<T, V, kNt, kTiled>), grid, dim3(kGnT), (2 * V + 1) * kGnT * sizeof(float), s, x, (float2*)ws, g);
+        STMI_LAUNCH_CHECK("gn_stats_kernel");
+        const float2* fold = (const float2*)ws;
+        if (!gn_folds_itself(g)) {
+            hipLaunchKernelGGL((gn_fold_kernel<kTiled>), gn_grid(ceil_div(groups, kGnT / 64), n), dim3(kGnT), 0, s, fold, stats, eps, g);
+            STMI_LAUNCH_CHECK("gn_fold_kernel");
+            fold = nullptr;
+        }
+        const int lds = (3 * c + 2 * groups) * (int)sizeof(float), most = 5 * STMI_GN_MAX_C * (int)sizeof(float);
+        if (residual) {
+            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, true, kTiled>), most, "gn_apply_kernel");
+            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, true, kTiled>), grid, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
+                               residual, y, act, g);
+        } else {
+            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, false, kTiled>), most, "gn_apply_kernel");
+            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, false, kTiled>), grid, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
+                               residual, y, act, g);
+        }
+        STMI_LAUNCH_CHECK("gn_apply_kernel");
+        return STMI_OK;
+    });
 }
 
 int gn_fwd_impl(const void* x, float* ws, float* stats, float eps, const float* scale, const float* shift,
@@ -675,27 +1255,51 @@ int gn_fwd_impl(const void* x, float* ws, float* stats, float eps, const float* 
 template <typename T, int V>
 static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* scale, const float* shift, T* dx, float* dscale,
                     float* dshift, int accumulate, float* ws, int act, int n, int P, int c, int groups, hipStream_t s) {
-    const GnGeom g = gn_geom(n, P, c, groups, V);
-    const long parts = (long)g.N * g.S * g.tiles;
-    float* rows = ws;
-    float* grows = rows + parts * 2 * g.C;
-    float* msums = grows + parts * 2 * g.G;
-    const int lds = (2 * V * kGnT + 2 * g.C) * (int)sizeof(float);
-    STMI_DYN_LDS((gn_bwd_sums_kernel<T, V>), (2 * V * kGnT + 2 * STMI_GN_MAX_C) * (int)sizeof(float), "gn_bwd_sums_kernel");
-    hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V>), dim3((unsigned)parts), dim3(kGnT), lds, s, x, dy, stats, scale, shift, rows, grows, act, g);
-    STMI_LAUNCH_CHECK("gn_bwd_sums_kernel");
-    const float* m = nullptr;
-    if (!gn_folds_itself(g)) {
-        hipLaunchKernelGGL(gn_fold_sums_kernel, dim3(g.N, ceil_div(g.G, kGnT / 64)), dim3(kGnT), 0, s, (const float*)grows, msums, g, 64);
-        STMI_LAUNCH_CHECK("gn_fold_sums_kernel");
-        m = msums;
+    GnGeom g = gn_geom(n, P, c, groups, V);
+    int threads, u;
+    if (gn_in_units(g, V, kGnUnitBwd, &threads, &u)) {
+        const int wide = g.D > V ? g.D : V;
+        const dim3 grid((unsigned)ceil_div((long)n * (c / wide), 8) * 8);
+        g.rQT = gn_recip(wide / V);
+        g.lgC = gn_lg_lanes(wide, threads);
+        float* r = dscale && n > 1 ? ws : nullptr;
+        gn_unit_launch<V>(g, u, [&](auto NS, auto U) {
+            hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads),
+                               2 * V * threads * sizeof(float), s, x, dy, stats, scale, shift, dx, r, dscale, dshift, accumulate, act, g);
+        });
+        STMI_LAUNCH_CHECK("gn_unit_bwd_kernel");
+        if (r) {
+            hipLaunchKernelGGL(gn_param_grads_kernel, dim3(ceil_div(2L * c, 64)), dim3(kGnT), 0, s, (const float*)r, (long)n, dscale,
+                               dshift, accumulate, c);
+            STMI_LAUNCH_CHECK("gn_param_grads_kernel");
+        }
+        return STMI_OK;
     }
-    const int pblocks = dscale ? ceil_div(2L * g.C, 64) : 0;
-    const int table = 2 * g.G > kGnT ? 2 * g.G : kGnT;
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V>), dim3((unsigned)(parts + pblocks)), dim3(kGnT), table * sizeof(float), s, x, dy,
-                       stats, scale, shift, (const float*)grows, m, (const float*)rows, dx, dscale, dshift, accumulate, act, g);
-    STMI_LAUNCH_CHECK("gn_bwd_apply_kernel");
-    return STMI_OK;
+    return gn_with_form(gn_streams(3, n, P, c, sizeof(T)), g, [&](auto NT, auto TL) -> int {
+        constexpr bool kNt = decltype(NT)::value, kTiled = decltype(TL)::value;
+        const long parts = (long)n * g.parts;
+        float* rows = ws;
+        float2* grows = (float2*)(rows + parts * 2 * c);
+        float* msums = (float*)(grows + parts * groups);
+        const int entries = 2 * V * kGnT, lds = ((entries > 3 * c ? entries : 3 * c) + 2 * c) * (int)sizeof(float);
+        STMI_DYN_LDS((gn_bwd_sums_kernel<T, V, kNt, kTiled>), 5 * STMI_GN_MAX_C * (int)sizeof(float), "gn_bwd_sums_kernel");
+        hipLaunchKernelGGL((gn_bwd_sums_kernel<T, V, kNt, kTiled>), gn_grid(g.parts, n), dim3(kGnT), lds, s, x, dy, stats, scale, shift,
+                           rows, grows, act, g);
+        STMI_LAUNCH_CHECK("gn_bwd_sums_kernel");
+        const float* m = nullptr;
+        if (!gn_folds_itself(g)) {
+            hipLaunchKernelGGL(gn_fold_sums_kernel, gn_grid(ceil_div(groups, kGnT / 64), n), dim3(kGnT), 0, s, (const float2*)grows, msums, g);
+            STMI_LAUNCH_CHECK("gn_fold_sums_kernel");
+            m = msums;
+        }
+        const int pblocks = dscale ? ceil_div(2L * c, 64) : 0, table = 5 * c + 2 * groups > kGnT ? 5 * c + 2 * groups : kGnT;
+        STMI_DYN_LDS((gn_bwd_apply_kernel<T, V, kNt, kTiled>), 7 * STMI_GN_MAX_C * (int)sizeof(float), "gn_bwd_apply_kernel");
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, kNt, kTiled>), gn_grid(g.parts + ceil_div(pblocks, n), n), dim3(kGnT),
+                           table * sizeof(float), s, x, dy, stats, scale, shift, (const float2*)grows, m, (const float*)rows, dx, dscale,
+                           dshift, accumulate, act, g);
+        STMI_LAUNCH_CHECK("gn_bwd_apply_kernel");
+        return STMI_OK;
+    });
 }
 
 int gn_bwd_impl(const void* x, const void* dy, const float* stats, const float* scale, const float* shift, void* dx,

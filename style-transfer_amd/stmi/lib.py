@@ -14,7 +14,7 @@ F32, BF16 = 0, 1
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3
 PACK_FWD, PACK_DGRAD, PACK_FWD_ROWOUT, PACK_FWD_RGB, PACK_DGRAD_RGB = 0, 1, 2, 3, 4
 LOSS_SLOT_FLOATS, LOSS_TERMS_MAX = 1024, 8
-GN_MAX_C, GRAD_WS_DOUBLES = 8192, 2048
+GN_MAX_C, GRAD_WS_DOUBLES = 4096, 2048
 
 _c_int, _c_long, _c_float, _vp = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p
 
@@ -71,7 +71,7 @@ SIGNATURES = {
     'stmi_instance_norm_nhwc_bwd_rows': (_c_int, [_vp] * 8 + [_c_int, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_instance_norm_bwd_rows_count': (_c_int, [_c_int] * 5),
     'stmi_instance_norm_param_grads': (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _vp, _c_int, _vp]),
-    'stmi_group_norm_ws_floats': (_c_long, [_c_int] * 6),
+    'stmi_group_norm_ws_floats': (_c_long, [_c_int] * 7),
     'stmi_group_norm_nhwc_fwd': (_c_int, [_vp, _vp, _vp, _c_float] + [_vp] * 4 + [_c_int] * 7 + [_vp]),
     'stmi_group_norm_nhwc_bwd': (_c_int, [_vp] * 8 + [_c_int, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_scale_shift': (_c_int, [_vp, _vp, _vp, _c_float, _c_long, _c_int, _c_int, _vp]),

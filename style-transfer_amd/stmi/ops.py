@@ -723,24 +723,38 @@ def _chk_out(out, name, like, *exact):
     return out
 
 
-def group_norm_ws(n, h, w, c, groups, dtype, device):
-    """Workspace of group_norm_fwd / group_norm_bwd for this geometry."""
+def group_norm_ws_floats(shape, groups, dtype, backward=False):
+    """Floats of workspace that group_norm_fwd (group_norm_bwd) uses for this geometry."""
     if dtype not in _DT:
         raise TypeError('stmi ops take float32 or bfloat16 tensors, got %s' % dtype)
-    need = _lib.load().stmi_group_norm_ws_floats(n, h, w, c, groups, _DT[dtype])
+    need = _lib.load().stmi_group_norm_ws_floats(*shape, groups, _DT[dtype], int(backward))
     if need < 0:
         raise _lib.StmiError(_lib.load().stmi_last_error().decode())
-    return torch.empty(max(need, 4), dtype=torch.float32, device=device)
+    return need
 
 
-def _group_norm_ws(ws, x, groups):
-    n, h, w, c = x.shape
+def _group_norm_ws(ws, x, groups, backward):
+    """The workspace's address (None where the call needs none) and what keeps it alive until the launch."""
+    need = group_norm_ws_floats(x.shape, groups, x.dtype, backward)
     if ws is None:
-        return group_norm_ws(n, h, w, c, groups, x.dtype, x.device)
-    _chk(ws, 'ws', torch.float32)
-    if ws.numel() < _lib.load().stmi_group_norm_ws_floats(n, h, w, c, groups, _dt(x)) or ws.data_ptr() % 16:
-        raise ValueError('ws must be 16-byte aligned and hold group_norm_ws(...) floats')
-    return ws
+        if need == 0:
+            return None, None
+        ws = torch.empty(need, dtype=torch.float32, device=x.device)
+    else:
+        _chk(ws, 'ws', torch.float32)
+        if ws.numel() < need or ws.data_ptr() % 16:
+            raise ValueError('ws must be 16-byte aligned and hold group_norm_ws_floats(...) = %d floats' % need)
+    return ws.data_ptr(), ws
+
+
+def _stream_on(dev):
+    """The current stream of device `dev` as _stream() gives it, without making a torch.cuda.Stream (0.1 us against 2.7)."""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _plain(t, dev, dtype, shape):
+    """What _chk asks for, and on device dev: one expression for the calls whose host time counts."""
+    return t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()
 
 
 def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None, out=None, stats=None, eps=IN_EPS):
@@ -748,20 +762,25 @@ def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None
     Returns (y, stats); stats [n,groups,2] = (mean, 1/sqrt(var+eps)) for group_norm_bwd.  out may be x or residual itself;
     any other overlap is not allowed.  act: ACT_NONE, ACT_RELU, ACT_SIGMOID or ACT_SILU."""
     n, h, w, c = x.shape
-    _chk(x, 'x')
-    _chk_here(x, 'x')
-    _chk(scale, 'scale', torch.float32, (c,))
-    _chk(shift, 'shift', torch.float32, (c,))
-    if residual is not None:
-        _chk(residual, 'residual', x.dtype, x.shape)
+    dev = torch.cuda.current_device() if x.is_cuda else -1
+    if not (_plain(x, dev, x.dtype, x.shape) and dev >= 0 and _plain(scale, dev, torch.float32, (c,))
+            and _plain(shift, dev, torch.float32, (c,)) and (residual is None or _plain(residual, dev, x.dtype, x.shape))):
+        _chk(x, 'x')
+        _chk(scale, 'scale', torch.float32, (c,))
+        _chk(shift, 'shift', torch.float32, (c,))
+        if residual is not None:
+            _chk(residual, 'residual', x.dtype, x.shape)
+        for t, nm in ((x, 'x'), (scale, 'scale'), (shift, 'shift'), (residual, 'residual')):
+            if t is not None:
+                _chk_here(t, nm)
+    wsp, ws = _group_norm_ws(ws, x, groups, False)
     y = torch.empty_like(x) if out is None else _chk_out(out, 'out', x, x, residual)
-    ws = _group_norm_ws(ws, x, groups)
     if stats is None:
         stats = torch.empty((n, groups, 2), dtype=torch.float32, device=x.device)
     else:
         _chk(stats, 'stats', torch.float32, (n, groups, 2))
-    _lib.call('stmi_group_norm_nhwc_fwd', x.data_ptr(), ws.data_ptr(), stats.data_ptr(), float(eps), scale.data_ptr(),
-              shift.data_ptr(), _ptr(residual), y.data_ptr(), act, n, h, w, c, groups, _dt(x), _stream())
+    _lib.call('stmi_group_norm_nhwc_fwd', x.data_ptr(), wsp, stats.data_ptr(), eps, scale.data_ptr(), shift.data_ptr(),
+              _ptr(residual), y.data_ptr(), act, n, h, w, c, groups, _DT[x.dtype], _stream_on(dev))
     return y, stats
 
 
@@ -770,20 +789,27 @@ def group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, act=ACT_N
     both None: not computed.  stats: what group_norm_fwd returned for x.  The gradient of a residual is dy.  out may be x or
     dy itself; any other overlap is not allowed."""
     n, h, w, c = x.shape
-    _chk(x, 'x')
-    _chk_here(x, 'x')
-    _chk(dy, 'dy', x.dtype, x.shape)
-    _chk(stats, 'stats', torch.float32, (n, groups, 2))
     if (dscale is None) != (dshift is None):
         raise ValueError('dscale and dshift are given together or not at all')
-    for t, nm in ((scale, 'scale'), (shift, 'shift'), (dscale, 'dscale'), (dshift, 'dshift')):
-        if t is not None:
-            _chk(t, nm, torch.float32, (c,))
-    ws = _group_norm_ws(ws, x, groups)
+    dev = torch.cuda.current_device() if x.is_cuda else -1
+    if not (_plain(x, dev, x.dtype, x.shape) and dev >= 0 and _plain(dy, dev, x.dtype, x.shape)
+            and _plain(stats, dev, torch.float32, (n, groups, 2)) and _plain(scale, dev, torch.float32, (c,))
+            and _plain(shift, dev, torch.float32, (c,))
+            and (dscale is None or _plain(dscale, dev, torch.float32, (c,)) and _plain(dshift, dev, torch.float32, (c,)))):
+        _chk(x, 'x')
+        _chk(dy, 'dy', x.dtype, x.shape)
+        _chk(stats, 'stats', torch.float32, (n, groups, 2))
+        for t, nm in ((scale, 'scale'), (shift, 'shift'), (dscale, 'dscale'), (dshift, 'dshift')):
+            if t is not None:
+                _chk(t, nm, torch.float32, (c,))
+        for t, nm in ((x, 'x'), (dy, 'dy'), (stats, 'stats'), (scale, 'scale'), (shift, 'shift'), (dscale, 'dscale'),
+                      (dshift, 'dshift')):
+            if t is not None:
+                _chk_here(t, nm)
+    wsp, ws = _group_norm_ws(ws, x, groups, True)
     dx = torch.empty_like(x) if out is None else _chk_out(out, 'out', x, x, dy)
     _lib.call('stmi_group_norm_nhwc_bwd', x.data_ptr(), dy.data_ptr(), stats.data_ptr(), scale.data_ptr(), shift.data_ptr(),
-              dx.data_ptr(), _ptr(dscale), _ptr(dshift), int(accumulate), ws.data_ptr(), act, n, h, w, c, groups, _dt(x),
-              _stream())
+              dx.data_ptr(), _ptr(dscale), _ptr(dshift), int(accumulate), wsp, act, n, h, w, c, groups, _DT[x.dtype], _stream_on(dev))
     return dx
 
 
@@ -990,7 +1016,8 @@ class GradList:
             _chk_here(o, 'output %d' % i)
         _chk_disjoint(tensors, outs)
         self._keep = (tensors, outs)
-        self.device = torch.device('cuda', torch.cuda.current_device())
+        self._dev = torch.cuda.current_device()
+        self.device = torch.device('cuda', self._dev)
         n, h = len(tensors), _lib.load()
         counts = (ctypes.c_long * n)(*[t.numel() for t in tensors])
         self._n = h.stmi_grad_list_chunks(counts, n)
@@ -999,31 +1026,38 @@ class GradList:
                   (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts,
                   (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors]), n, table)
         self._table = torch.frombuffer(table, dtype=torch.uint8).to(self.device)
+        self._place = self._table.data_ptr()
         self._ws = torch.empty(_lib.GRAD_WS_DOUBLES, dtype=torch.float64, device=self.device)
+        self._ws_place = self._ws.data_ptr()
+
+    def _chk_current(self):
+        if torch.cuda.current_device() != self._dev:
+            raise ValueError('the list lives on cuda:%d, not on the current device' % self._dev)
 
     def _norm_out(self, out):
-        _chk_here(self._table, 'the list')
+        self._chk_current()
         if out is None:
             return torch.empty(1, dtype=torch.float32, device=self.device)
-        return _chk(out, 'norm', torch.float32, (1,))
+        _chk_here(_chk(out, 'norm', torch.float32, (1,)), 'norm')
+        return out
 
     def sum_squares(self):
         """Leaves the sum of squares (as partial sums) for adam_tf1(..., clip=self)."""
-        _chk_here(self._table, 'the list')
-        _lib.call('stmi_grad_sum_squares', self._table.data_ptr(), self._n, self._ws.data_ptr(), _stream())
+        self._chk_current()
+        _lib.call('stmi_grad_sum_squares', self._place, self._n, self._ws_place, _stream_on(self._dev))
 
     def norm(self, out=None):
         """The global L2 norm, fp32 [1] on the device."""
         out = self._norm_out(out)
-        _lib.call('stmi_grad_norm', self._table.data_ptr(), self._n, self._ws.data_ptr(), out.data_ptr(), _stream())
+        _lib.call('stmi_grad_norm', self._place, self._n, self._ws_place, out.data_ptr(), _stream_on(self._dev))
         return out
 
     def clip(self, max_norm, norm=None):
         """outs = tensors * max_norm / max(norm, max_norm); returns the norm before clipping, fp32 [1] on the device.  A norm
         that is not finite makes every output NaN."""
         norm = self._norm_out(norm)
-        _lib.call('stmi_grad_clip', self._table.data_ptr(), self._n, self._ws.data_ptr(), float(max_norm), norm.data_ptr(),
-                  _stream())
+        _lib.call('stmi_grad_clip', self._place, self._n, self._ws_place, float(max_norm), norm.data_ptr(),
+                  _stream_on(self._dev))
         return norm
 
 
@@ -1045,11 +1079,11 @@ def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, s
         t = 0 if advance else -1
     if clip is not None:
         _chk_here(p, 'p')
-        _chk_here(clip._table, 'clip')
+        clip._chk_current()
         if norm is not None:
             _chk(norm, 'norm', torch.float32, (1,))
         _lib.call('stmi_adam_tf1_clip', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
-                  float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws.data_ptr(), float(max_norm), _ptr(norm),
+                  float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws_place, float(max_norm), _ptr(norm),
                   _ptr(step_dev), int(t), _stream())
         return
     _lib.call('stmi_adam_tf1', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),

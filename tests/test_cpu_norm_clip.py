@@ -9,10 +9,14 @@ import torch
 def test_group_norm_arguments():
     from stmi import lib
     h = lib.load()
-    ws = lambda *a: h.stmi_group_norm_ws_floats(*a)   # noqa: E731
-    assert ws(2, 8, 8, 64, 8, lib.F32) >= 0 and ws(0, 8, 8, 64, 8, lib.BF16) >= 0
+    ws = lambda *a: h.stmi_group_norm_ws_floats(*a, 0)   # noqa: E731
+    assert ws(2, 256, 256, 64, 8, lib.F32) > 0 and ws(0, 8, 8, 64, 8, lib.BF16) == 0
+    # one block per group: no workspace forward; a row of sums per sample backward, none for one sample
+    assert ws(2, 8, 8, 64, 8, lib.BF16) == 0
+    assert [h.stmi_group_norm_ws_floats(n, 8, 8, 64, 8, lib.BF16, 1) for n in (1, 3)] == [0, 3 * 2 * 64]
+    assert h.stmi_group_norm_nhwc_fwd(1, None, 1, 1e-3, 1, 1, None, 1, 0, 2, 256, 256, 64, 8, 0, None) == -1
     for bad in ((2, 8, 8, 64, 7, 0), (2, 8, 8, 64, 0, 0), (2, 8, 8, 64, -8, 0), (2, 0, 8, 64, 8, 0), (2, 8, 0, 64, 8, 0),
-                (-1, 8, 8, 64, 8, 0), (2, 8, 8, 0, 8, 0), (2, 8, 8, 64, 8, 2), (2, 8, 8, 8193, 1, 0), (1, 65536, 32768, 8, 1, 0)):
+                (-1, 8, 8, 64, 8, 0), (2, 8, 8, 0, 8, 0), (2, 8, 8, 64, 8, 2), (2, 8, 8, 4097, 1, 0), (1, 65536, 32768, 8, 1, 0)):
         assert ws(*bad) == -1, bad
         assert h.stmi_last_error()
     fwd = lambda act, *a: h.stmi_group_norm_nhwc_fwd(1, 1, 1, 1e-3, 1, 1, None, 1, act, *a, None)   # noqa: E731

@@ -93,14 +93,24 @@ SHAPES = [  # n, h, w, c, groups
     (1, 1, 1, 8, 2), (1, 1, 1, 1, 1), (2, 1, 1, 512, 32), (3, 1, 7, 3, 1), (1, 5, 3, 3, 3),
     (2, 16, 16, 512, 32), (2, 17, 23, 32, 8), (1, 64, 48, 128, 32), (2, 33, 31, 64, 64), (1, 40, 41, 64, 1),
     (2, 13, 27, 35, 5), (1, 19, 21, 101, 101), (1, 9, 11, 257, 1), (2, 7, 5, 1000, 8), (1, 3, 5, 2040, 8),
-    (1, 2, 3, 8192, 32), (1, 3, 3, 8190, 2), (1, 2, 2, 4099, 1), (5, 6, 7, 24, 12), (2, 50, 40, 16, 16), (17, 3, 3, 96, 3),
+    (1, 2, 3, 4096, 32), (1, 3, 3, 4094, 2), (1, 2, 2, 4093, 1), (1, 40, 50, 4096, 4096), (2, 30, 31, 4095, 4095), (5, 6, 7, 24, 12), (2, 50, 40, 16, 16), (17, 3, 3, 96, 3),
     (1, 200, 150, 12, 3), (3, 45, 67, 20, 2), (1, 130, 110, 256, 32),
+    # one block per group: full and over-full registers, columns that do not divide the block
+    (3, 64, 64, 64, 32), (3, 32, 32, 48, 2), (2, 37, 30, 72, 3), (1, 63, 43, 120, 5), (1, 65, 64, 64, 16), (9, 1, 2, 64, 64),
+    (1, 8, 8, 1024, 2), (2, 45, 45, 16, 2),
 ]
+
+
+@pytest.fixture(params=['chosen', 'slices'])
+def form(request, monkeypatch):
+    """The form the library chooses (small samples: one block per group), and the one that cuts samples into slices."""
+    if request.param == 'slices':
+        monkeypatch.setenv('STMI_NO_GN_UNITS', '1')
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('shape', SHAPES, ids=lambda s: 'x'.join(map(str, s)))
-def test_forward_and_backward(cuda, shape, dtype):
+def test_forward_and_backward(cuda, shape, dtype, form):
     from stmi import ops
     *dims, groups = shape
     act = [ops.ACT_SILU, ops.ACT_NONE, ops.ACT_SIGMOID, ops.ACT_RELU][(dims[1] + dims[3]) % 4]
@@ -131,7 +141,7 @@ def test_forward_and_backward(cuda, shape, dtype):
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('act', ['NONE', 'RELU', 'SIGMOID', 'SILU'])
 @pytest.mark.parametrize('shape', [(2, 12, 20, 64, 16), (2, 70, 90, 32, 8), (1, 11, 13, 35, 7)], ids=lambda s: 'x'.join(map(str, s)))
-def test_every_activation_with_residual(cuda, shape, act, dtype):
+def test_every_activation_with_residual(cuda, shape, act, dtype, form):
     from stmi import ops
     *dims, groups = shape
     act = getattr(ops, 'ACT_' + act)
@@ -181,7 +191,7 @@ def test_groups_equal_to_channels_is_the_instance_norm(cuda):
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('mean,dev', [(300.0, 1.0), (0.0, 1e-4), (0.0, 1e6)], ids=['mean', 'small', 'large'])
 @pytest.mark.parametrize('shape', [(2, 16, 16, 64, 8), (1, 96, 100, 64, 8)], ids=lambda s: 'x'.join(map(str, s)))
-def test_means_and_deviations_of_other_sizes(cuda, shape, mean, dev, dtype):
+def test_means_and_deviations_of_other_sizes(cuda, shape, mean, dev, dtype, form):
     from stmi import ops
     *dims, groups = shape
     x, scale, shift, _, _ = data(dims, dtype, 8, mean, dev)
@@ -192,7 +202,7 @@ def test_means_and_deviations_of_other_sizes(cuda, shape, mean, dev, dtype):
 
 @pytest.mark.parametrize('where', ['first', 'last', 'middle'])
 @pytest.mark.parametrize('shape', [(1, 16, 16, 64, 8), (1, 128, 128, 32, 4)], ids=lambda s: 'x'.join(map(str, s)))
-def test_one_far_value(cuda, shape, where):
+def test_one_far_value(cuda, shape, where, form):
     """One value 1e5 deviations away, at a place a shifted sum might take as its shift."""
     from stmi import ops
     *dims, groups = shape
@@ -207,7 +217,7 @@ def test_one_far_value(cuda, shape, where):
 
 @pytest.mark.parametrize('shape', [(3, 8, 8, 64, 8), (3, 72, 80, 32, 4), (2, 9, 7, 35, 5)], ids=lambda s: 'x'.join(map(str, s)))
 @pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')], ids=['nan', 'inf', '-inf'])
-def test_not_finite_values_stay_in_their_group(cuda, shape, bad):
+def test_not_finite_values_stay_in_their_group(cuda, shape, bad, form):
     from stmi import ops
     *dims, groups = shape
     x, scale, shift, dy, _ = data(dims, torch.bfloat16, 4)
@@ -229,7 +239,7 @@ def test_not_finite_values_stay_in_their_group(cuda, shape, bad):
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('hw', [(4, 4), (90, 100)], ids=['small', 'large'])
-def test_constant_groups(cuda, hw, dtype):
+def test_constant_groups(cuda, hw, dtype, form):
     from stmi import ops
     x = torch.full((2,) + hw + (32,), 3.3, dtype=dtype, device=cuda)
     scale, shift = torch.ones(32, device=cuda), torch.full((32,), 0.5, device=cuda)
@@ -244,7 +254,7 @@ def test_constant_groups(cuda, hw, dtype):
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('shape', [(5, 16, 16, 128, 32), (3, 120, 130, 32, 8), (3, 11, 13, 35, 5), (3, 45, 61, 35, 5)], ids=lambda s: 'x'.join(map(str, s)))
-def test_a_sample_does_not_depend_on_its_batch_and_bits_repeat(cuda, shape, dtype):
+def test_a_sample_does_not_depend_on_its_batch_and_bits_repeat(cuda, shape, dtype, form):
     from stmi import ops
     *dims, groups = shape
     x, scale, shift, dy, _ = (t.to(cuda) for t in data(dims, dtype, 6))
@@ -260,7 +270,7 @@ def test_a_sample_does_not_depend_on_its_batch_and_bits_repeat(cuda, shape, dtyp
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
 @pytest.mark.parametrize('shape', [(2, 16, 16, 64, 8), (2, 110, 100, 32, 8), (2, 13, 9, 35, 5)], ids=lambda s: 'x'.join(map(str, s)))
-def test_places(cuda, shape, dtype):
+def test_places(cuda, shape, dtype, form):
     """Outputs in the inputs' own memory, and tensors at any element of a larger buffer (the values around stay)."""
     from stmi import ops
     *dims, groups = shape
@@ -394,7 +404,7 @@ def test_refusals(cuda):
     with pytest.raises(lib.StmiError, match='bad activation'):
         ops.group_norm_fwd(x, 2, s, s, act=4)
     with pytest.raises(lib.StmiError, match='channels'):
-        ops.group_norm_fwd(torch.zeros((1, 1, 1, 8193), device=cuda), 1, torch.ones(8193, device=cuda), torch.ones(8193, device=cuda))
+        ops.group_norm_fwd(torch.zeros((1, 1, 1, 4097), device=cuda), 1, torch.ones(4097, device=cuda), torch.ones(4097, device=cuda))
     with pytest.raises(TypeError):
         ops.group_norm_fwd(x.half(), 2, s, s)
     with pytest.raises(TypeError):
@@ -409,7 +419,7 @@ def test_refusals(cuda):
     with pytest.raises(ValueError, match='overlaps'):
         ops.group_norm_fwd(buf[:-8].view(x.shape), 2, s, s, out=buf[8:].view(x.shape))
     with pytest.raises(ValueError, match='ws'):
-        ops.group_norm_fwd(x, 2, s, s, ws=torch.empty(0, device=cuda))
+        ops.group_norm_fwd(torch.zeros((1, 256, 256, 8), device=cuda), 2, s, s, ws=torch.empty(0, device=cuda))
     y, stats = ops.group_norm_fwd(x, 2, s, s)
     with pytest.raises(ValueError, match='together'):
         ops.group_norm_bwd(x, x, 2, stats, s, s, s.clone(), None)
