@@ -472,7 +472,7 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count,
  * writes it to HOST memory (no launch), the caller copies it to the device and keeps it for as long as the tensors
  * (srcs) and the outputs (dsts, elementwise the same shapes and types; dsts[i] may be srcs[i], no other overlap) stay
  * where they are.  Tensors of length zero have no chunks.
- * ws: STMI_GRAD_WS_DOUBLES doubles of scratch; a call overwrites it entirely.  Calls that share a ws must be ordered.
+ * ws: STMI_GRAD_WS_DOUBLES doubles of scratch.  Calls that share a ws must be ordered.
  * stmi_grad_sum_squares : leaves partial sums of squares in ws for stmi_adam_tf1_clip.
  * stmi_grad_norm        : the same, and norm (device fp32 [1]).
  * stmi_grad_clip        : the same, and the outputs; norm (may be NULL) is the norm BEFORE clipping.  Where dsts[i] is
@@ -483,7 +483,7 @@ typedef struct {
     void* dst;
     int count, dtype;
 } stmi_grad_chunk;
-long stmi_grad_list_chunks(const long* counts, int n);
+long stmi_grad_list_chunks(const long* counts, const int* dtypes, int n);
 int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
                         stmi_grad_chunk* host_table);
 int stmi_grad_sum_squares(const stmi_grad_chunk* table, int nchunks, double* ws, void* stream);
@@ -491,10 +491,10 @@ int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float*
 int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream);
 /* stmi_adam_tf1 of gradients clipped on the way in: g * grad_scale is scaled by max_norm / max(norm, max_norm) with
  * norm = |grad_scale| * sqrt(sum of the partial sums in ws), as stmi_grad_sum_squares left them for all gradients that
- * share the norm.  norm (device fp32 [1], may be NULL) receives it. */
+ * share the norm (nchunks: that call's).  norm (device fp32 [1], may be NULL) receives it. */
 int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count,
                        float lr, float beta1, float beta2, float eps, float grad_scale,
-                       const double* ws, float max_norm, float* norm, int* step_dev, int t, void* stream);
+                       const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t, void* stream);
 
 /* ---- row patches for layers with < 8 channels on one side (the 9x9 RGB layers) ----------
  * A kw x c window of an NHWC tensor is kw*c contiguous elements.  Copying it once per pixel

@@ -127,14 +127,15 @@ int gram_mse_impl(const float*, const float*, void*, float*, float, float, int, 
 int tv_impl(const float*, void*, float*, float, int, int, int, int, int, hipStream_t);
 int loss_slots_sum_impl(const float* slots, const int* first, int nterms, float* out, hipStream_t s);
 int adam_impl(float*, const float*, float*, float*, long, float, float, float, float, float, int*, int, hipStream_t);
-long grad_list_chunks(const long* counts, int n);
+long grad_list_chunks(const long* counts, const int* dtypes, int n);
 void grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
                     stmi_grad_chunk* table);
 int grad_squares_impl(const stmi_grad_chunk* table, int nchunks, double* ws, hipStream_t s);
-int grad_norm_impl(const double* ws, float* norm, hipStream_t s);
+int grad_norm_impl(const double* ws, int nchunks, float* norm, hipStream_t s);
 int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws, float max_norm, float* norm, hipStream_t s);
 int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, float lr, float b1, float b2, float eps,
-                   float grad_scale, const double* ws, float max_norm, float* norm, int* step_dev, int t, hipStream_t s);
+                   float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t,
+                   hipStream_t s);
 
 static int check_dtype(int dtype) {
     if (dtype == STMI_F32 || dtype == STMI_BF16) return STMI_OK;
@@ -725,11 +726,11 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count, floa
     return adam_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, step_dev, t, S(stream));
 }
 
-long stmi_grad_list_chunks(const long* counts, int n) {
-    if (!counts && n > 0) return -1;
+long stmi_grad_list_chunks(const long* counts, const int* dtypes, int n) {
+    if (n < 0 || (n > 0 && !(counts && dtypes))) return -1;
     for (int i = 0; i < n; i++)
         if (counts[i] < 0) return -1;
-    return grad_list_chunks(counts, n);
+    return grad_list_chunks(counts, dtypes, n);
 }
 
 int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* counts, const int* dtypes, int n,
@@ -741,7 +742,7 @@ int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* 
         const uintptr_t size = dtypes[i] == STMI_BF16 ? 2 : 4;
         STMI_REQUIRE((uintptr_t)srcs[i] % size == 0 && (uintptr_t)dsts[i] % size == 0, "grad_list_fill: tensor %d is not aligned to its elements", i);
     }
-    const long chunks = grad_list_chunks(counts, n);
+    const long chunks = grad_list_chunks(counts, dtypes, n);
     STMI_REQUIRE(chunks == 0 || host_table, "grad_list_fill: null table");
     STMI_REQUIRE(chunks < (1L << 31), "grad_list_fill: more than 2^31 chunks");
     grad_list_fill(srcs, dsts, counts, dtypes, n, host_table);
@@ -756,7 +757,7 @@ int stmi_grad_sum_squares(const stmi_grad_chunk* table, int nchunks, double* ws,
 int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float* norm, void* stream) {
     STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws && norm, "grad_norm: bad arguments");
     const int rc = grad_squares_impl(table, nchunks, ws, S(stream));
-    return rc ? rc : grad_norm_impl(ws, norm, S(stream));
+    return rc ? rc : grad_norm_impl(ws, nchunks, norm, S(stream));
 }
 
 int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream) {
@@ -767,12 +768,12 @@ int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float 
 }
 
 int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count, float lr, float beta1, float beta2,
-                       float eps, float grad_scale, const double* ws, float max_norm, float* norm, int* step_dev, int t,
-                       void* stream) {
-    STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws, "adam_tf1_clip: bad arguments");
+                       float eps, float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev,
+                       int t, void* stream) {
+    STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws && nchunks >= 0, "adam_tf1_clip: bad arguments");
     STMI_REQUIRE(step_dev || t >= 1, "adam_tf1_clip: step t must be >= 1 (got %d)", t);
     STMI_REQUIRE(max_norm > 0.f && max_norm <= 3.402823466e38f, "adam_tf1_clip: max_norm must be finite and > 0 (got %g)", (double)max_norm);
-    return adam_clip_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, ws, max_norm, norm, step_dev, t, S(stream));
+    return adam_clip_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, ws, nchunks, max_norm, norm, step_dev, t, S(stream));
 }
 
 int stmi_cast(const void* src, void* dst, long count, int dtype, int to_f32, void* stream) {

@@ -1020,11 +1020,11 @@ class GradList:
         self.device = torch.device('cuda', self._dev)
         n, h = len(tensors), _lib.load()
         counts = (ctypes.c_long * n)(*[t.numel() for t in tensors])
-        self._n = h.stmi_grad_list_chunks(counts, n)
+        dtypes = (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors])
+        self._n = h.stmi_grad_list_chunks(counts, dtypes, n)
         table = (_lib.GradChunk * max(self._n, 1))()
         _lib.call('stmi_grad_list_fill', (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-                  (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts,
-                  (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors]), n, table)
+                  (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts, dtypes, n, table)
         self._table = torch.frombuffer(table, dtype=torch.uint8).to(self.device)
         self._place = self._table.data_ptr()
         self._ws = torch.empty(_lib.GRAD_WS_DOUBLES, dtype=torch.float64, device=self.device)
@@ -1083,8 +1083,8 @@ def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, s
         if norm is not None:
             _chk(norm, 'norm', torch.float32, (1,))
         _lib.call('stmi_adam_tf1_clip', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
-                  float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws_place, float(max_norm), _ptr(norm),
-                  _ptr(step_dev), int(t), _stream())
+                  float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws_place, clip._n, float(max_norm),
+                  _ptr(norm), _ptr(step_dev), int(t), _stream())
         return
     _lib.call('stmi_adam_tf1', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
               float(beta1), float(beta2), float(eps), float(grad_scale), _ptr(step_dev), int(t), _stream())

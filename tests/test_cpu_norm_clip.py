@@ -34,7 +34,7 @@ def fill(lengths, dtypes, src, dst):
     from stmi import lib
     h, n = lib.load(), len(lengths)
     counts = (ctypes.c_long * n)(*lengths)
-    k = h.stmi_grad_list_chunks(counts, n)
+    k = h.stmi_grad_list_chunks(counts, (ctypes.c_int * n)(*dtypes), n)
     table = (lib.GradChunk * max(k, 1))()
     rc = h.stmi_grad_list_fill((ctypes.c_void_p * n)(*src), (ctypes.c_void_p * n)(*dst), counts, (ctypes.c_int * n)(*dtypes), n, table)
     return rc, [(c.src, c.dst, c.count, c.dtype) for c in table[:k]]
@@ -64,15 +64,15 @@ def test_chunk_table_refusals():
     assert fill([4], [1], [16], [17])[0] == -1
     assert fill([4], [0], [None], [16])[0] == -1
     assert fill([0], [0], [None], [None]) == (0, [])
-    assert h.stmi_grad_list_chunks((ctypes.c_long * 1)(-1), 1) == -1
+    assert h.stmi_grad_list_chunks((ctypes.c_long * 1)(-1), (ctypes.c_int * 1)(0), 1) == -1
     assert h.stmi_grad_clip(None, 3, 1, 1.0, None, None) == -1
     assert h.stmi_grad_norm(1, 3, 1, None, None) == -1
     assert h.stmi_grad_sum_squares(1, -1, 1, None) == -1
     for bad in (0.0, -2.0, float('inf'), float('nan')):
         assert h.stmi_grad_clip(1, 3, 1, bad, None, None) == -1 and b'max_norm' in h.stmi_last_error()
-        assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, 1, bad, None, None, 1, None) == -1
-    assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, 1, 1.0, None, None, 0, None) == -1
-    assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, None, 1.0, None, None, 1, None) == -1
+        assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, 1, 3, bad, None, None, 1, None) == -1
+    assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, 1, 3, 1.0, None, None, 0, None) == -1
+    assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, None, 3, 1.0, None, None, 1, None) == -1
 
 
 def test_overlapping_outputs_are_refused():
