@@ -14,9 +14,9 @@ namespace stmi {
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 constexpr int kChunkBytes = 16384, kVecs = kChunkBytes / 16 / 256;   // 16-byte accesses of a thread
-// Chunks from which the tensors (read) and the outputs (written) exceed the last-level cache together (256 MB): the outputs
-// then go past it, so that the second reading of the tensors still finds them there.
-constexpr int kStreamChunks = (128 << 20) / kChunkBytes;
+// Chunks (32 MB) from which the outputs go past the caches: the second reading of the tensors then still finds them in the
+// last-level cache (600 ragged tensors, 223 MB read and written: 71 us with ordinary stores, 57 without).
+constexpr int kStreamChunks = (32 << 20) / kChunkBytes;
 
 template <bool kNt>
 __device__ __forceinline__ u32x4 load16(const void* p) {

@@ -41,6 +41,7 @@ struct GnGeom {
     int L, Q, R;         // elements and V-wide columns of a row, whole rows of a sample
     int QT, tiles;       // columns a block owns, blocks side by side in a row
     int S, rows;         // slices of a sample, rows of a slice
+    int S2, rows2;       // the same for the second launch
     int slots;           // rows a block walks at once (one tile)
     int parts;           // S * tiles: partial results of a sample, blocks of a sample
     int lgG, lgC;        // log2 of the lanes that reduce one group, one channel
@@ -172,7 +173,8 @@ struct GnPlace {
     long first;        // the slice's first element
     long end0;         // the tail's first element
     unsigned own;      // the thread's first element in the slice
-    __device__ __forceinline__ GnPlace(const GnGeom& g, int V) {
+    bool last;         // the last slice: the tail is its
+    __device__ __forceinline__ GnPlace(const GnGeom& g, int V, int S, int slice_rows) {
         n = gn_sample();
         s = blockIdx.x;
         tile = c0 = 0;
@@ -189,15 +191,15 @@ struct GnPlace {
             slot = gn_div(threadIdx.x, g.rQT);
         }
         col = c0 + threadIdx.x - slot * QT;
-        const int r0 = min(s * g.rows, g.R);
-        rows = min(g.rows, g.R - r0);
+        const int r0 = min(s * slice_rows, g.R);
+        rows = min(slice_rows, g.R - r0);
+        last = s == S - 1 && tile == 0;
         const long base = (long)n * g.P * g.C;
         first = base + (long)r0 * g.L;
         end0 = base + (long)g.R * g.L;
         own = slot * g.L + col * V;
     }
     __device__ __forceinline__ bool on() const { return slot < slots; }
-    __device__ __forceinline__ bool owns_tail(const GnGeom& g) const { return s == g.S - 1 && tile == 0; }
     __device__ __forceinline__ long part(const GnGeom& g) const { return (long)n * g.parts + blockIdx.x; }
 };
 
@@ -232,7 +234,7 @@ template <typename T, int V, bool kNt, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ ws, const GnGeom g) {
     constexpr int kB = 8;
     extern __shared__ float sh[];   // [V][kGnT] means, [V][kGnT] sums of squares, [kGnT] counts
-    const GnPlace<kTiled> p(g, V);
+    const GnPlace<kTiled> p(g, V, g.S, g.rows);
     if (p.n >= g.N) return;
     float mean[V], m2[V];
 #pragma unroll
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
                     f(lc[t], lm[j * kGnT + t], l2[j * kGnT + t]);
                 }
             }
-            if (g.tail && p.owns_tail(g)) {
+            if (g.tail && p.last) {
                 for (int e = lane; e < g.tail / g.C * g.D; e += K)
                     f(1.f, to_f32<T>(x[p.end0 + e / g.D * g.C + gr * g.D + e % g.D]), 0.f);
             }
@@ -419,14 +421,14 @@ __global__ __launch_bounds__(kGnT) void gn_fold_kernel(const float2* __restrict_
 // A slice is walked from its end: what the first launch read last is the likeliest to be in a cache still.  The loads of a
 // thread's first rows are on their way while the block folds the partials and makes its table (mean, scale * rstd, shift of
 // every channel), those of the next rows while it computes.
-template <typename T, int V, bool kNt, bool kRes, bool kTiled>
+template <typename T, int V, bool kNt, bool kPut, bool kRes, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const float2* __restrict__ ws, float* __restrict__ stats,
                                                         float eps, const float* __restrict__ scale,
                                                         const float* __restrict__ shift, const T* residual, T* y, int act,
                                                         const GnGeom g) {
     constexpr int kU = 4;
     extern __shared__ float tab[];   // [3][C] mean, scale * rstd, shift; [2G]
-    const GnPlace<kTiled> p(g, V);
+    const GnPlace<kTiled> p(g, V, g.S2, g.rows2);
     if (p.n >= g.N) return;
     const int batch = p.slots * kU, full = p.rows / batch, rest = p.rows - full * batch;
     const int step = p.slots * g.L;
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const flo
 #pragma unroll
                     for (int j = 0; j < V; j++) v[j] += r[j];
                 }
-                gn_store<kNt, T, V>(y + where, own, v);
+                gn_store<kPut, T, V>(y + where, own, v);
             };
             u32x4 res[kU];
             if (p.slot < rest) {
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const flo
                 for (int u = 0; u < kU; u++) put(raw[u], res[u], at + u * (long)step);
             }
         }
-        if (g.tail && p.owns_tail(g)) {
+        if (g.tail && p.last) {
             for (int e = threadIdx.x; e < g.tail; e += kGnT) {
                 const long q = p.end0 + e;
                 const int c = e % g.C;
@@ -538,10 +540,10 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_sums_kernel(const T* __restric
                                                            const float* __restrict__ stats, const float* __restrict__ scale,
                                                            const float* __restrict__ shift, float* __restrict__ rows,
                                                            float2* __restrict__ grows, int act, const GnGeom g) {
-    constexpr int kB = 4;
+    constexpr int kB = 2;
     extern __shared__ float sh[];   // [3][C] mean, scale * rstd, shift, then [V][kGnT] sums of g, [V][kGnT] of g (x - mean);
                                     // behind the larger of the two: [2][C] the block's sums per channel
-    const GnPlace<kTiled> p(g, V);
+    const GnPlace<kTiled> p(g, V, g.S, g.rows);
     if (p.n >= g.N) return;
     const float* st = stats + (long)p.n * g.G * 2;
     for (int c = threadIdx.x; c < g.C; c += kGnT) {
@@ -581,30 +583,28 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_sums_kernel(const T* __restric
                     s2[j] += gv * xm;
                 }
             };
-            const T* xb = x + p.first;
-            const T* db = dy + p.first;
-            int left = p.rows;
-            u32x4 vr[kB], dr[kB];
-            for (; left >= batch; left -= batch, xb += kB * (long)step, db += kB * (long)step) {
-#pragma unroll
-                for (int u = 0; u < kB; u++) {
-                    vr[u] = gn_load<kNt>(xb + u * (long)step, own);
-                    dr[u] = gn_load<kNt>(db + u * (long)step, own);
-                }
-#pragma unroll
-                for (int u = 0; u < kB; u++) add(vr[u], dr[u]);
-            }
-            if (p.slot < left) {   // the last, shorter batch
+            // two batches of rows: one on its way, one in the computation
+            u32x4 vr[kB], dr[kB], vn[kB], dn[kB];
+            auto load = [&](u32x4 (&v)[kB], u32x4 (&d)[kB], int left, long at) {
 #pragma unroll
                 for (int u = 0; u < kB; u++) {
                     if (p.slot < left - u * p.slots) {
-                        vr[u] = gn_load<kNt>(xb + u * (long)step, own);
-                        dr[u] = gn_load<kNt>(db + u * (long)step, own);
+                        v[u] = gn_load<kNt>(x + at + u * (long)step, own);
+                        d[u] = gn_load<kNt>(dy + at + u * (long)step, own);
                     }
                 }
+            };
+            long at = p.first;
+            load(vr, dr, p.rows, at);
+            for (int left = p.rows; left > 0; left -= batch) {
+                at += kB * (long)step;
+                load(vn, dn, left - batch, at);
 #pragma unroll
-                for (int u = 0; u < kB; u++)
+                for (int u = 0; u < kB; u++) {
                     if (p.slot < left - u * p.slots) add(vr[u], dr[u]);
+                    vr[u] = vn[u];
+                    dr[u] = dn[u];
+                }
             }
         }
 #pragma unroll
@@ -629,7 +629,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_sums_kernel(const T* __restric
                         t2 += l2[j * kGnT + slot * p.QT + col];
                     }
                 }
-                if (g.tail && p.owns_tail(g)) {
+                if (g.tail && p.last) {
                     for (int e = lane; e < g.tail / g.C; e += K) {
                         const long q = p.end0 + e * g.C + c;
                         const float xm = to_f32<T>(x[q]) - st[2 * gr];
@@ -727,7 +727,7 @@ __device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, l
 // ------------------------------------------------------------------ backward, second launch
 // The last blocks fold the parameter gradients, the others write dx.  As in the forward pass a slice is walked from its
 // end, and loads are on their way during the fold and the computation of the rows before.
-template <typename T, int V, bool kNt, bool kTiled>
+template <typename T, int V, bool kNt, bool kPut, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const T* dy, const float* __restrict__ stats,
                                                             const float* __restrict__ scale, const float* __restrict__ shift,
                                                             const float2* __restrict__ grows, const float* __restrict__ msums,
@@ -737,12 +737,13 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
     // [5][C] mean, scale * rstd, shift, k1 = rstd m1, k2 = rstd^2 m2 with dx = scale rstd g - k1 - (x - mean) k2; [2G] m1, m2
     // (512 floats at least)
     extern __shared__ float tab[];
-    if ((int)blockIdx.x >= g.parts) {
-        const long q = (long)(blockIdx.x - g.parts) * g.N + gn_sample();
+    const int blocks2 = g.S2 * g.tiles;
+    if ((int)blockIdx.x >= blocks2) {
+        const long q = (long)(blockIdx.x - blocks2) * g.N + gn_sample();
         if (gn_sample() < g.N && q * 64 < 2 * g.C) gn_param_grads(rows, (long)g.N * g.parts, dscale, dshift, accumulate, g.C, (int)q, tab);
         return;
     }
-    const GnPlace<kTiled> p(g, V);
+    const GnPlace<kTiled> p(g, V, g.S2, g.rows2);
     if (p.n >= g.N) return;
     const int batch = p.slots * kU, full = p.rows / batch, rest = p.rows - full * batch;
     const int step = p.slots * g.L;
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
                     const float xm = v[j] - mean[j];
                     v[j] = d[j] * gn_act_grad<kA>(xm * a[j] + bb[j]) * a[j] - k1[j] - xm * k2[j];
                 }
-                gn_store<kNt, T, V>(dx + where, own, v);
+                gn_store<kPut, T, V>(dx + where, own, v);
             };
             if (p.slot < rest) {
 #pragma unroll
@@ -833,7 +834,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
                 for (int u = 0; u < kU; u++) put(vr[u], dr[u], at + u * (long)step);
             }
         }
-        if (g.tail && p.owns_tail(g)) {
+        if (g.tail && p.last) {
             for (int e = threadIdx.x; e < g.tail; e += kGnT) {
                 const long q = p.end0 + e;
                 const int c = e % g.C;
@@ -1108,7 +1109,7 @@ static unsigned gn_recip(int d) { return d == 1 ? 0u : (unsigned)(((1UL << 32) +
 
 static int gcd_int(int a, int b) { return b ? gcd_int(b, a % b) : a; }
 
-static GnGeom gn_geom(int n, int P, int c, int groups, int V) {
+static GnGeom gn_geom(int n, int P, int c, int groups, int V, bool backward) {
     GnGeom g;
     g.N = n; g.P = P; g.C = c; g.G = groups; g.D = c / groups;
     g.L = c / gcd_int(c, V) * V;
@@ -1123,8 +1124,8 @@ static GnGeom gn_geom(int n, int P, int c, int groups, int V) {
     g.lgC = gn_lg_lanes(c, kGnT);
     // A sample is cut the same way whatever its batch: slices of four rows a thread (32 KB) for the smaller samples, up to
     // kGnSlices larger ones for the larger.
-    const int per4 = g.R / (g.slots * 4);
-    int S = per4 < 128 ? per4 : per4 < 256 ? 128 : per4 / 2;
+    const int per4 = g.R / (g.slots * 4), per8 = g.R / (g.slots * 8), most4 = backward ? 128 : 64;
+    int S = per8 < most4 ? (per4 < most4 ? per4 : most4) : per8;
     // few enough partials for the second launch to fold, unless the sample is large (32 MB) or would be cut in too few
     const int few = (kGnFoldLane << g.lgG) / g.tiles;
     if (S > few && few >= 64 && (long)P * c / V * 16 <= (32L << 20)) S = few;
@@ -1135,6 +1136,17 @@ static GnGeom gn_geom(int n, int P, int c, int groups, int V) {
     g.S = ceil_div(g.R, g.rows);
     if (g.S < 1) g.S = 1;
     g.parts = g.S * g.tiles;
+    // The second launch's cut changes no sum: one block a CU where its fold and table are a good part of the work, several
+    // where the tensor is large, four rows a thread at least.
+    const long mb = (long)n * P * c / V * 16 >> 20;
+    const int blocks2 = mb > 256 ? 2048 : mb > 48 || backward ? 512 : 256;
+    int S2 = ceil_div(blocks2, (long)(n > 0 ? n : 1) * g.tiles);
+    if (S2 > per4) S2 = per4;
+    if (S2 < 1) S2 = 1;
+    g.rows2 = ceil_div(g.R, S2);
+    if (g.rows2 < 1) g.rows2 = 1;
+    g.S2 = ceil_div(g.R, g.rows2);
+    if (g.S2 < 1) g.S2 = 1;
     const int units = g.D / g.U, entries = units * (g.L / c), K = 1 << g.lgG;
     g.over_slots = entries * ceil_div(g.slots, K) <= g.slots * ceil_div(entries, K);
     g.rC = gn_recip(c);
@@ -1170,7 +1182,7 @@ static bool gn_in_units(const GnGeom& g, int V, int most_threads, int* threads, 
 
 long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward) {
     const int V = dtype == STMI_BF16 ? 8 : 4;
-    const GnGeom g = gn_geom(n, h * w, c, groups, V);
+    const GnGeom g = gn_geom(n, h * w, c, groups, V, backward);
     const long parts = (long)n * g.parts;
     int threads, u;
     if (gn_in_units(g, V, backward ? kGnUnitBwd : kGnUnitFwd, &threads, &u)) return backward && n > 1 ? (long)n * 2 * c : 0;
@@ -1192,21 +1204,32 @@ static void gn_unit_launch(const GnGeom& g, int u, F&& f) {
     else with_u(std::integral_constant<int, V>{});
 }
 
-// Tensors that together exceed the last-level cache (256 MB) are streamed past it.
-static bool gn_streams(int tensors, int n, int P, int c, int size) { return (long)tensors * n * P * c * size > (256L << 20); }
+// Streaming past the caches.  Outputs do from 64 MB of tensors on (below that the next operator may find them in the L2s):
+// what was read stays in the last-level cache (256 MB) for the second launch.  16 x 540 x 960 x 32 bf16 cut to 1, 3 and 4
+// samples, forward: 22.9 / 63 / 82 us with ordinary stores, 21.3 / 54 / 71 without.  Inputs that do not fit that cache are
+// not kept in it either: a 2.1 GB tensor is read at 7.1 TB/s instead of 6.2.
+struct GnStream {
+    bool loads, stores;
+    GnStream(int read, int others, int n, int P, int c, int size) {
+        const long one = (long)n * P * c * size;
+        loads = read * one > (224L << 20);
+        stores = (read + others) * one > (64L << 20);
+    }
+};
 
-// f(kNt, kTiled) as compile-time constants; rows of several tiles are rare (odd channel counts above 512): one form
+// f(kNt, kPut, kTiled) as compile-time constants; rows of several tiles are rare (odd channel counts above 512): one form
 template <typename F>
-static int gn_with_form(bool nt, const GnGeom& g, F&& f) {
-    if (g.tiles > 1) return f(std::false_type{}, std::true_type{});
-    if (nt) return f(std::true_type{}, std::false_type{});
-    return f(std::false_type{}, std::false_type{});
+static int gn_with_form(const GnStream& st, const GnGeom& g, F&& f) {
+    if (g.tiles > 1) return f(std::false_type{}, std::false_type{}, std::true_type{});
+    if (st.loads) return f(std::true_type{}, std::true_type{}, std::false_type{});
+    if (st.stores) return f(std::false_type{}, std::true_type{}, std::false_type{});
+    return f(std::false_type{}, std::false_type{}, std::false_type{});
 }
 
 template <typename T, int V>
 static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float* scale, const float* shift, const T* residual,
                     T* y, int act, int n, int P, int c, int groups, hipStream_t s) {
-    GnGeom g = gn_geom(n, P, c, groups, V);
+    GnGeom g = gn_geom(n, P, c, groups, V, false);
     int threads, u;
     if (gn_in_units(g, V, kGnUnitFwd, &threads, &u)) {
         const int wide = g.D > V ? g.D : V;
@@ -1219,9 +1242,9 @@ static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float*
         STMI_LAUNCH_CHECK("gn_unit_fwd_kernel");
         return STMI_OK;
     }
-    return gn_with_form(gn_streams(residual ? 3 : 2, n, P, c, sizeof(T)), g, [&](auto NT, auto TL) -> int {
-        constexpr bool kNt = decltype(NT)::value, kTiled = decltype(TL)::value;
-        const dim3 grid = gn_grid(g.parts, n);
+    return gn_with_form(GnStream(1, residual ? 2 : 1, n, P, c, sizeof(T)), g, [&](auto NT, auto PT, auto TL) -> int {
+        constexpr bool kNt = decltype(NT)::value, kPut = decltype(PT)::value, kTiled = decltype(TL)::value;
+        const dim3 grid = gn_grid(g.parts, n), grid2 = gn_grid(g.S2 * g.tiles, n);
         hipLaunchKernelGGL((gn_stats_kernel<T, V, kNt, kTiled>), grid, dim3(kGnT), (2 * V + 1) * kGnT * sizeof(float), s, x, (float2*)ws, g);
         STMI_LAUNCH_CHECK("gn_stats_kernel");
         const float2* fold = (const float2*)ws;
@@ -1232,12 +1255,12 @@ static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float*
         }
         const int lds = (3 * c + 2 * groups) * (int)sizeof(float), most = 5 * STMI_GN_MAX_C * (int)sizeof(float);
         if (residual) {
-            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, true, kTiled>), most, "gn_apply_kernel");
-            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, true, kTiled>), grid, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
+            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, kPut, true, kTiled>), most, "gn_apply_kernel");
+            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, kPut, true, kTiled>), grid2, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
                                residual, y, act, g);
         } else {
-            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, false, kTiled>), most, "gn_apply_kernel");
-            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, false, kTiled>), grid, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
+            STMI_DYN_LDS((gn_apply_kernel<T, V, kNt, kPut, false, kTiled>), most, "gn_apply_kernel");
+            hipLaunchKernelGGL((gn_apply_kernel<T, V, kNt, kPut, false, kTiled>), grid2, dim3(kGnT), lds, s, x, fold, stats, eps, scale, shift,
                                residual, y, act, g);
         }
         STMI_LAUNCH_CHECK("gn_apply_kernel");
@@ -1255,7 +1278,7 @@ int gn_fwd_impl(const void* x, float* ws, float* stats, float eps, const float* 
 template <typename T, int V>
 static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* scale, const float* shift, T* dx, float* dscale,
                     float* dshift, int accumulate, float* ws, int act, int n, int P, int c, int groups, hipStream_t s) {
-    GnGeom g = gn_geom(n, P, c, groups, V);
+    GnGeom g = gn_geom(n, P, c, groups, V, true);
     int threads, u;
     if (gn_in_units(g, V, kGnUnitBwd, &threads, &u)) {
         const int wide = g.D > V ? g.D : V;
@@ -1275,8 +1298,8 @@ static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* sc
         }
         return STMI_OK;
     }
-    return gn_with_form(gn_streams(3, n, P, c, sizeof(T)), g, [&](auto NT, auto TL) -> int {
-        constexpr bool kNt = decltype(NT)::value, kTiled = decltype(TL)::value;
+    return gn_with_form(GnStream(2, 1, n, P, c, sizeof(T)), g, [&](auto NT, auto PT, auto TL) -> int {
+        constexpr bool kNt = decltype(NT)::value, kPut = decltype(PT)::value, kTiled = decltype(TL)::value;
         const long parts = (long)n * g.parts;
         float* rows = ws;
         float2* grows = (float2*)(rows + parts * 2 * c);
@@ -1293,8 +1316,8 @@ static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* sc
             m = msums;
         }
         const int pblocks = dscale ? ceil_div(2L * c, 64) : 0, table = 5 * c + 2 * groups > kGnT ? 5 * c + 2 * groups : kGnT;
-        STMI_DYN_LDS((gn_bwd_apply_kernel<T, V, kNt, kTiled>), 7 * STMI_GN_MAX_C * (int)sizeof(float), "gn_bwd_apply_kernel");
-        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, kNt, kTiled>), gn_grid(g.parts + ceil_div(pblocks, n), n), dim3(kGnT),
+        STMI_DYN_LDS((gn_bwd_apply_kernel<T, V, kNt, kPut, kTiled>), 7 * STMI_GN_MAX_C * (int)sizeof(float), "gn_bwd_apply_kernel");
+        hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, kNt, kPut, kTiled>), gn_grid(g.S2 * g.tiles + ceil_div(pblocks, n), n), dim3(kGnT),
                            table * sizeof(float), s, x, dy, stats, scale, shift, (const float2*)grows, m, (const float*)rows, dx, dscale,
                            dshift, accumulate, act, g);
         STMI_LAUNCH_CHECK("gn_bwd_apply_kernel");
