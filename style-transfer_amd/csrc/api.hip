@@ -607,6 +607,7 @@ int stmi_group_norm_nhwc_fwd(const void* x, float* ws, float* stats, float eps, 
                              const void* residual, void* y, int act, int n, int h, int w, int c, int groups, int dtype,
                              void* stream) {
     if (check_group_norm("group_norm_nhwc_fwd", act, n, h, w, c, groups, dtype)) return STMI_ERR_INVALID;
+    STMI_REQUIRE(eps >= 1e-30f && eps <= 3.402823466e38f, "group_norm_nhwc_fwd: eps must be finite and at least 1e-30 (got %g)", (double)eps);
     if (n == 0) return STMI_OK;
     STMI_REQUIRE(x && stats && scale && shift && y && (ws || gn_ws_floats(n, h, w, c, groups, dtype, 0) == 0),
                  "group_norm_nhwc_fwd: bad arguments");

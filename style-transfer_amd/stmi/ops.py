@@ -974,34 +974,34 @@ def tv_loss_fwd_bwd(img_f32, loss, weight, dtype, out=None):
 def _chk_disjoint(tensors, outs):
     """An output may be its own tensor; any other overlap of an output with a tensor or an output is refused: chunks are
     read and written in no order."""
-    spans = []
-    for i, (t, o) in enumerate(zip(tensors, outs)):
-        if t.numel():
-            nbytes = t.numel() * t.element_size()
-            spans.append((t.data_ptr(), t.data_ptr() + nbytes, 0, i))
-            spans.append((o.data_ptr(), o.data_ptr() + nbytes, 1, i))
-    reach = [(0, -1), (0, -1)]          # the two tensors that reach furthest so far, of different indexes
-    last = (0, 0, -1)                   # the output that reaches furthest so far (outputs are disjoint)
-    for start, end, is_out, i in sorted(spans):
-        if is_out:
-            clash = last[1] > start
-            for e, j in reach:
-                clash = clash or (e > start and j != i)
-            clash = clash or any(e > start and j == i for e, j in reach) and tensors[i].data_ptr() != start
-            last = (start, end, i)
-        else:
-            clash = last[1] > start and not (last[2] == i and last[0] == start)
-            reach = sorted(reach + [(end, i)], reverse=True)[:2]
-        if clash:
-            raise ValueError('output or tensor %d overlaps another one' % i)
+    import numpy as np
+    idx = [i for i, t in enumerate(tensors) if t.numel()]
+    if not idx:
+        return
+    size = np.array([tensors[i].numel() * tensors[i].element_size() for i in idx], np.int64)
+    o0 = np.array([outs[i].data_ptr() for i in idx], np.int64)
+    order = np.argsort(o0, kind='stable')
+    a, e = o0[order], (o0 + size)[order]
+    hit = np.nonzero(e[:-1] > a[1:])[0]
+    if hit.size:
+        raise ValueError('output %d overlaps another output' % idx[order[hit[0] + 1]])
+    if outs is tensors:
+        return
+    t0 = np.array([tensors[i].data_ptr() for i in idx], np.int64)
+    # the outputs (sorted, disjoint) that tensor k touches are first[k] .. last[k] - 1: none, or its own in the same place
+    first, last = np.searchsorted(e, t0, 'right'), np.searchsorted(a, t0 + size, 'left')
+    own = (last - first == 1) & (order[np.minimum(first, len(idx) - 1)] == np.arange(len(idx))) & (o0 == t0)
+    bad = np.nonzero((last > first) & ~own)[0]
+    if bad.size:
+        raise ValueError('an output overlaps tensor %d' % idx[bad[0]])
 
 
 class GradList:
     """The gradients of a training step as ONE list: their global norm, and clipping by it, in one launch each however
     many there are.  tensors: contiguous fp32 / bf16 tensors of any lengths on the current device; outs: what clip() writes,
     tensor by tensor (default: the tensors themselves).  The list keeps the tensors, their places (a device table built
-    here, once) and a workspace: build it before a graph that uses it is captured, keep it as long as the graph, and order
-    its calls (two graphs that may run at the same time need a list each)."""
+    here, once) and a workspace: build it before a graph that uses it is captured, keep it as long as the graph and until its
+    work has ended, and order its calls (two graphs that may run at the same time need a list each)."""
 
     def __init__(self, tensors, outs=None):
         import ctypes
@@ -1009,14 +1009,15 @@ class GradList:
         outs = tensors if outs is None else list(outs)
         if len(outs) != len(tensors):
             raise ValueError('%d tensors, but %d outputs' % (len(tensors), len(outs)))
+        self._dev = torch.cuda.current_device() if torch.cuda.is_available() else 0
         for i, (t, o) in enumerate(zip(tensors, outs)):
-            _dt(_chk(t, 'tensor %d' % i))
-            _chk_here(t, 'tensor %d' % i)
-            _chk(o, 'output %d' % i, t.dtype, t.shape)
-            _chk_here(o, 'output %d' % i)
+            if not (_plain(t, self._dev, t.dtype, t.shape) and t.dtype in _DT and (o is t or _plain(o, self._dev, t.dtype, t.shape))):
+                _dt(_chk(t, 'tensor %d' % i))
+                _chk_here(t, 'tensor %d' % i)
+                _chk(o, 'output %d' % i, t.dtype, t.shape)
+                _chk_here(o, 'output %d' % i)
         _chk_disjoint(tensors, outs)
         self._keep = (tensors, outs)
-        self._dev = torch.cuda.current_device()
         self.device = torch.device('cuda', self._dev)
         n, h = len(tensors), _lib.load()
         counts = (ctypes.c_long * n)(*[t.numel() for t in tensors])

@@ -24,6 +24,9 @@ def test_group_norm_arguments():
     assert fwd(-1, 2, 8, 8, 64, 8, 0) == -1
     assert fwd(0, 2, 8, 8, 64, 24, 0) == -1 and b'multiple' in h.stmi_last_error()
     assert fwd(0, 2, 8, 8, 64, 8, 5) == -1 and b'dtype' in h.stmi_last_error()
+    for eps in (0.0, -1e-3, float('nan'), float('inf')):
+        assert h.stmi_group_norm_nhwc_fwd(1, 1, 1, eps, 1, 1, None, 1, 0, 2, 8, 8, 64, 8, 0, None) == -1
+        assert b'eps' in h.stmi_last_error()
     assert h.stmi_group_norm_nhwc_fwd(None, 1, 1, 1e-3, 1, 1, None, 1, 0, 2, 8, 8, 64, 8, 0, None) == -1
     assert h.stmi_group_norm_nhwc_fwd(None, None, None, 1e-3, None, None, None, None, 0, 0, 8, 8, 64, 8, 0, None) == 0   # empty batch
     bwd = lambda x, ds, dh: h.stmi_group_norm_nhwc_bwd(x, 1, 1, 1, 1, 1, ds, dh, 0, 1, 0, 2, 8, 8, 64, 8, 0, None)   # noqa: E731
@@ -88,6 +91,13 @@ def test_overlapping_outputs_are_refused():
     for ts, outs in bad:
         with pytest.raises(ValueError, match='overlaps'):
             _chk_disjoint(ts, outs)
+    for same in ([a, a], [a, a[:1]], [a, a[99:]], [b, a[:60], a[40:]]):
+        with pytest.raises(ValueError, match='overlaps'):
+            _chk_disjoint(same, same)
+    pieces = [a[i:i + 1] for i in range(100)]
+    _chk_disjoint(pieces[::-1], pieces[::-1])
+    with pytest.raises(ValueError, match='overlaps'):
+        _chk_disjoint(pieces, pieces[::-1])
 
 
 def test_product_path_refuses_cpu_tensors():

@@ -301,6 +301,54 @@ def test_trainer_clips_to_the_global_norm(cuda):
         trainer(max_grad_norm=0.0)
 
 
+class TwoEqualRanks:
+    """Gradient buckets of a group of two ranks with equal gradients: a bucket holds the sum once it has been waited for,
+    and not before."""
+
+    def __init__(self, flat, ranges):
+        self.flat, self.ranges, self.pending, self.log = flat, list(ranges), set(), []
+        self.replay_seconds, self.replays, self.steps = 0.0, 0, 0
+
+    def reduce_bucket(self, i):
+        self.pending.add(i)
+
+    def wait_bucket(self, i):
+        if i in self.pending:
+            self.pending.remove(i)
+            self.log.append(i)
+            self.flat[slice(*self.ranges[i])].mul_(2.0)
+
+    def wait(self):
+        for i in sorted(self.pending):
+            self.wait_bucket(i)
+
+
+@pytest.mark.parametrize('use_graph', [False, True], ids=['eager', 'graph'])
+def test_data_parallel_trainer_clips_the_mean_of_all_buckets(cuda, use_graph, monkeypatch):
+    import numpy as np
+    import torch.distributed as dist
+    from oracle import tf_ops as O
+    from stmi import trainer as T
+    monkeypatch.setattr(dist, 'barrier', lambda group=None: None)
+    rng = np.random.default_rng(1)
+    batch = torch.tensor(rng.random((1, 32, 32, 3)).astype(np.float32), device=cuda)
+    style = torch.tensor(rng.random((1, 32, 32, 3)).astype(np.float32))
+    make = lambda **kw: T.StyleTrainer(1, 32, 32, cuda, O.synthetic_vgg_weights(seed=5, width_div=8), np.zeros(3, np.float32),   # noqa: E731
+                                       1e3, 1.0, 10.0, params=O.init_stylizer_params(seed=3), max_grad_norm=0.5, **kw)
+    one, two = make(use_graph=False), make(use_graph=use_graph)
+    assert len(T.BWD_SEGMENTS) > 1
+    two.world = 2
+    two.buckets = TwoEqualRanks(two.net.flat_grad, [two.net.param_range(hi, lo) for hi, lo in T.BWD_SEGMENTS])
+    for t in (one, two):
+        t.set_style_image(style)
+        for _ in range(2):
+            t.step(batch)
+    torch.cuda.synchronize()
+    assert one.grad_norm.item() > 1.0
+    # the mean of two equal gradients is the gradient: same norm, same update (doubling and halving are exact)
+    assert torch.equal(one.grad_norm, two.grad_norm) and torch.equal(one.net.flat, two.net.flat)
+
+
 def test_refusals(cuda):
     from stmi import lib, ops
     t = torch.zeros(100, device=cuda)

@@ -98,6 +98,8 @@ SHAPES = [  # n, h, w, c, groups
     # one block per group: full and over-full registers, columns that do not divide the block
     (3, 64, 64, 64, 32), (3, 32, 32, 48, 2), (2, 37, 30, 72, 3), (1, 63, 43, 120, 5), (1, 65, 64, 64, 16), (9, 1, 2, 64, 64),
     (1, 8, 8, 1024, 2), (2, 45, 45, 16, 2),
+    # partials folded by a launch of their own: many groups, a large sample
+    (1, 200, 200, 128, 128), (1, 513, 520, 64, 32),
 ]
 
 
@@ -379,6 +381,20 @@ def test_captured_and_replayed_on_another_stream(cuda, shape):
     torch.cuda.current_stream().wait_stream(side)
     for a, b in zip(got, step(x, dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('c,groups', [(3, 1), (8, 2)])
+def test_more_samples_than_a_grid_dimension(cuda, c, groups):
+    from stmi import ops
+    n = 70001
+    x, scale, shift, dy, _ = (t.to(cuda) for t in data((n, 2, 3, c), torch.float32, 40))
+    f = formula(x.cpu(), groups, scale.cpu(), shift.cpu(), ops.ACT_SILU, dy=dy.cpu())
+    y, stats = ops.group_norm_fwd(x, groups, scale, shift, act=ops.ACT_SILU, eps=EPS)
+    near(y, f['y'], 1.1 * f['dz'])
+    gs, gh = torch.zeros((2, c), device=cuda)
+    near(ops.group_norm_bwd(x, dy, groups, stats, scale, shift, gs, gh, act=ops.ACT_SILU), f['dx'], f['dx_tol'])
+    near(gs, f['dscale'], f['dscale_tol'])
+    near(gh, f['dshift'], f['dshift_tol'])
 
 
 def test_empty_batch(cuda):
