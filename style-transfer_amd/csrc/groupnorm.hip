@@ -1122,31 +1122,26 @@ static GnGeom gn_geom(int n, int P, int c, int groups, int V, bool backward) {
     g.tail = (int)((long)P * c - (long)g.R * g.L);
     g.lgG = gn_lg_lanes(groups, kGnT);
     g.lgC = gn_lg_lanes(c, kGnT);
-    // A sample is cut the same way whatever its batch: slices of four rows a thread (32 KB) for the smaller samples, up to
-    // kGnSlices larger ones for the larger.
-    const int per4 = g.R / (g.slots * 4), per8 = g.R / (g.slots * 8), most4 = backward ? 128 : 64;
-    int S = per8 < most4 ? (per4 < most4 ? per4 : most4) : per8;
+    // `deep` rows a thread of a sample, cut into slices of k: the same way whatever its batch.  Four to eight rows (32 to 64
+    // KB a slice): with fewer rows, more blocks for a lone sample; with more, fewer fixed costs (fold, tables, reductions)
+    // for a batch.  Forward, 1 and 16 samples of 256 x 256 x 32 bf16: four rows 9.9 and 40.6 us, eight 10.1 and 35.6;
+    // backward (with forward) 21.5 and 110, 25.3 and 98.6.
+    const int deep = ceil_div(g.R, g.slots), most = backward ? 128 : 64;
+    int k = deep <= 4 * most ? 4 : deep <= 8 * most ? ceil_div(deep, most) : 8;
     // few enough partials for the second launch to fold, unless the sample is large (32 MB) or would be cut in too few
-    const int few = (kGnFoldLane << g.lgG) / g.tiles;
-    if (S > few && few >= 64 && (long)P * c / V * 16 <= (32L << 20)) S = few;
-    if (S > kGnSlices / g.tiles) S = kGnSlices / g.tiles;
-    if (S < 1) S = 1;
-    g.rows = ceil_div(g.R, S);
-    if (g.rows < 1) g.rows = 1;
-    g.S = ceil_div(g.R, g.rows);
-    if (g.S < 1) g.S = 1;
+    const int few = (kGnFoldLane << g.lgG) / g.tiles, all = kGnSlices / g.tiles;
+    if (few >= 64 && (long)P * c / V * 16 <= (32L << 20) && k < ceil_div(deep, few)) k = ceil_div(deep, few);
+    if (k < ceil_div(deep, all)) k = ceil_div(deep, all);
+    g.rows = g.slots * k;
+    g.S = g.R ? ceil_div(g.R, g.rows) : 1;
     g.parts = g.S * g.tiles;
     // The second launch's cut changes no sum: one block a CU where its fold and table are a good part of the work, several
     // where the tensor is large, four rows a thread at least.
     const long mb = (long)n * P * c / V * 16 >> 20;
     const int blocks2 = mb > 256 ? 2048 : mb > 48 || backward ? 512 : 256;
-    int S2 = ceil_div(blocks2, (long)(n > 0 ? n : 1) * g.tiles);
-    if (S2 > per4) S2 = per4;
-    if (S2 < 1) S2 = 1;
-    g.rows2 = ceil_div(g.R, S2);
-    if (g.rows2 < 1) g.rows2 = 1;
-    g.S2 = ceil_div(g.R, g.rows2);
-    if (g.S2 < 1) g.S2 = 1;
+    const int k2 = ceil_div((long)deep * g.tiles * (n > 0 ? n : 1), blocks2);
+    g.rows2 = g.slots * (k2 > 4 ? k2 : 4);
+    g.S2 = g.R ? ceil_div(g.R, g.rows2) : 1;
     const int units = g.D / g.U, entries = units * (g.L / c), K = 1 << g.lgG;
     g.over_slots = entries * ceil_div(g.slots, K) <= g.slots * ceil_div(entries, K);
     g.rC = gn_recip(c);
