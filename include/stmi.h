@@ -493,7 +493,7 @@ int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float 
  * norm = |grad_scale| * sqrt(sum of the partial sums in ws), as stmi_grad_sum_squares left them for all gradients that
  * share the norm (nchunks: that call's).  norm (device fp32 [1], may be NULL) receives it. */
 int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count,
-                       float lr, float beta1, float beta2, float eps, float grad_scale,
+                       double lr, double beta1, double beta2, float eps, float grad_scale,
                        const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t, void* stream);
 
 /* ---- row patches for layers with < 8 channels on one side (the 9x9 RGB layers) ----------

@@ -133,7 +133,7 @@ void grad_list_fill(const void* const* srcs, void* const* dsts, const long* coun
 int grad_squares_impl(const stmi_grad_chunk* table, int nchunks, double* ws, hipStream_t s);
 int grad_norm_impl(const double* ws, int nchunks, float* norm, hipStream_t s);
 int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws, float max_norm, float* norm, hipStream_t s);
-int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, float lr, float b1, float b2, float eps,
+int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, double lr, double b1, double b2, float eps,
                    float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t,
                    hipStream_t s);
 
@@ -768,7 +768,7 @@ int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float 
     return rc ? rc : grad_scale_impl(table, nchunks, ws, max_norm, norm, S(stream));
 }
 
-int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count, float lr, float beta1, float beta2,
+int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count, double lr, double beta1, double beta2,
                        float eps, float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev,
                        int t, void* stream) {
     STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws && nchunks >= 0, "adam_tf1_clip: bad arguments");

@@ -211,7 +211,8 @@ int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws,
 
 // ------------------------------------------------------------------ Adam with clipping
 // The update of stmi_adam_tf1 with g' = g * grad_scale * factor, factor from the norm of g * grad_scale: clipping costs
-// no pass of its own.  28 bytes a parameter; four parameters a thread and access, and the loads of a thread's first ones
+// no pass of its own.  The rates come in double: 1 - beta2 and 1 - beta2^t of an fp32 0.999 are 1.3e-5 off, and the step
+// with them.  28 bytes a parameter; four parameters a thread and access, and the loads of a thread's first ones
 // are on their way while the block folds the partial sums and one thread of its last wave works out the step size.
 
 // b^t for t >= 0 by squaring: t times 2^-53 off at most, and shorter than two pow()
@@ -224,8 +225,8 @@ __device__ __forceinline__ double pow_int(double b, unsigned t) {
 
 template <bool kNt>
 __global__ __launch_bounds__(256) void adam_clip_kernel(float* __restrict__ p, const float* __restrict__ g,
-                                                        float* __restrict__ m, float* __restrict__ v, long count, float lr,
-                                                        float b1, float b2, float eps, float grad_scale,
+                                                        float* __restrict__ m, float* __restrict__ v, long count, double lr,
+                                                        double beta1, double beta2, float eps, float grad_scale,
                                                         const double* __restrict__ ws, int nparts, float max_norm,
                                                         float* __restrict__ norm_out, const int* step_dev, int t_host) {
     __shared__ double red[4];
@@ -241,15 +242,16 @@ __global__ __launch_bounds__(256) void adam_clip_kernel(float* __restrict__ p, c
     }
     if (threadIdx.x == 255) {
         const unsigned t = step_dev ? step_dev[0] : t_host;
-        sh = (float)((double)lr * sqrt(1.0 - pow_int(b2, t)) / (1.0 - pow_int(b1, t)));
+        sh = (float)(lr * sqrt(1.0 - pow_int(beta2, t)) / (1.0 - pow_int(beta1, t)));
     }
+    const float b1 = (float)beta1, b2 = (float)beta2, c1 = (float)(1.0 - beta1), c2 = (float)(1.0 - beta2);
     const double norm = sqrt(fold_squares(ws, nparts, red)) * fabs((double)grad_scale);   // its barrier is sh's too
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
     const float lr_t = sh, gs = grad_scale * clip_factor(norm, max_norm);
     auto update = [&](float gi, float& mi, float& vi, float& pi) {
         gi *= gs;
-        mi = b1 * mi + (1.f - b1) * gi;
-        vi = b2 * vi + (1.f - b2) * gi * gi;
+        mi = b1 * mi + c1 * gi;
+        vi = b2 * vi + c2 * gi * gi;
         pi -= lr_t * mi / (sqrtf(vi) + eps);
     };
     for (bool first = true; q < quads; q += stride, first = false) {
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(256) void adam_clip_kernel(float* __restrict__ p, c
 
 __global__ void bump_step_kernel(int* step);
 
-int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, float lr, float b1, float b2, float eps,
+int adam_clip_impl(float* p, const float* g, float* m, float* v, long count, double lr, double b1, double b2, float eps,
                    float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t,
                    hipStream_t s) {
     if (step_dev && t >= 0) {

@@ -166,7 +166,7 @@ static dim3 gn_grid(int parts, int n) {
 }
 
 // a block's sample, slice and column tile, and what the calling thread owns of the tile.  kTiled: a row has more columns
-// than a block has threads (odd channel counts above 512 only)
+// than a block has threads
 template <bool kTiled>
 struct GnPlace {
     int n, s, tile, c0, QT, slots, col, slot, rows;
@@ -1184,19 +1184,23 @@ long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backwar
     return backward ? parts * 2 * c + parts * 2 * groups + (long)n * 2 * groups : parts * 2 * groups;
 }
 
-// f(groups of a column, vectors of a thread) as compile-time constants
-template <int V, typename F>
+// f(groups of a column, vectors of a thread) as compile-time constants.  Units 16 bytes wide have 2048 vectors at most
+// (gn_in_units): two a thread forward (1024 threads), two or four backward (512).
+template <int V, int kNarrow, typename F>
 static void gn_unit_launch(const GnGeom& g, int u, F&& f) {
-    auto with_u = [&](auto NS) {
-        if (u == 2) f(NS, std::integral_constant<int, 2>{});
-        else if (u == 4) f(NS, std::integral_constant<int, 4>{});
-        else f(NS, std::integral_constant<int, 8>{});
-    };
     const int ns = g.D >= V ? 1 : V / g.D;
-    if (ns == 1) with_u(std::integral_constant<int, 1>{});
-    else if (ns == 2) with_u(std::integral_constant<int, 2>{});
-    else if (ns == 4) with_u(std::integral_constant<int, 4>{});
-    else with_u(std::integral_constant<int, V>{});
+    auto narrow = [&](auto NS) {
+        if (kNarrow == 2 || u == 2) f(NS, std::integral_constant<int, 2>{});
+        else f(NS, std::integral_constant<int, kNarrow>{});
+    };
+    if (ns == 1) {
+        std::integral_constant<int, 1> one;
+        if (u == 2) f(one, std::integral_constant<int, 2>{});
+        else if (u == 4) f(one, std::integral_constant<int, 4>{});
+        else f(one, std::integral_constant<int, 8>{});
+    } else if (ns == 2) narrow(std::integral_constant<int, 2>{});
+    else if (ns == 4) narrow(std::integral_constant<int, 4>{});
+    else narrow(std::integral_constant<int, V>{});
 }
 
 // Streaming past the caches.  Outputs do from 64 MB of tensors on (below that the next operator may find them in the L2s):
@@ -1212,7 +1216,8 @@ struct GnStream {
     }
 };
 
-// f(kNt, kPut, kTiled) as compile-time constants; rows of several tiles are rare (odd channel counts above 512): one form
+// f(kNt, kPut, kTiled) as compile-time constants; rows of several tiles are rare (more than 512
+// columns: channel counts above 512 V, or above 512 and no multiple of V): one form
 template <typename F>
 static int gn_with_form(const GnStream& st, const GnGeom& g, F&& f) {
     if (g.tiles > 1) return f(std::false_type{}, std::false_type{}, std::true_type{});
@@ -1230,7 +1235,7 @@ static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float*
         const int wide = g.D > V ? g.D : V;
         const dim3 grid((unsigned)ceil_div((long)n * (c / wide), 8) * 8);
         g.rQT = gn_recip(wide / V);
-        gn_unit_launch<V>(g, u, [&](auto NS, auto U) {
+        gn_unit_launch<V, 2>(g, u, [&](auto NS, auto U) {
             hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads), 0, s, x, stats,
                                eps, scale, shift, residual, y, act, g);
         });
@@ -1281,7 +1286,7 @@ static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* sc
         g.rQT = gn_recip(wide / V);
         g.lgC = gn_lg_lanes(wide, threads);
         float* r = dscale && n > 1 ? ws : nullptr;
-        gn_unit_launch<V>(g, u, [&](auto NS, auto U) {
+        gn_unit_launch<V, 4>(g, u, [&](auto NS, auto U) {
             hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads),
                                2 * V * threads * sizeof(float), s, x, dy, stats, scale, shift, dx, r, dscale, dshift, accumulate, act, g);
         });

@@ -93,7 +93,7 @@ SIGNATURES = {
     'stmi_grad_sum_squares': (_c_int, [_vp, _c_int, _vp, _vp]),
     'stmi_grad_norm': (_c_int, [_vp, _c_int] + [_vp] * 3),
     'stmi_grad_clip': (_c_int, [_vp, _c_int, _vp, _c_float, _vp, _vp]),
-    'stmi_adam_tf1_clip': (_c_int, [_vp] * 4 + [_c_long] + [_c_float] * 5 + [_vp, _c_int, _c_float, _vp, _vp, _c_int, _vp]),
+    'stmi_adam_tf1_clip': (_c_int, [_vp] * 4 + [_c_long] + [ctypes.c_double] * 3 + [_c_float] * 2 + [_vp, _c_int, _c_float, _vp, _vp, _c_int, _vp]),
     'stmi_cast': (_c_int, [_vp, _vp, _c_long, _c_int, _c_int, _vp]),
     'stmi_pixels_to_rows': (_c_int, [_vp, _vp] + [_c_int] * 7 + [_vp]),
     'stmi_rows_to_pixels_sum': (_c_int, [_vp, _vp, _vp] + [_c_int] * 7 + [_vp]),

@@ -3,8 +3,7 @@
 Tolerances, before any run (u = 2^-24, half a step of fp32).  Squares of fp32 and bf16 values are summed in double, where a
 product rounds by 2^-53: the norm is off by its one rounding to fp32, u (2 u allowed).  The factor rounds once (u), its
 product with a gradient once more (u, or 2^-8 to bf16): 3 u resp. 2^-8 + 3 u of an output's value.  Adam: m and v are sums
-of two products, (1 - b1) and (1 - b2) are taken of fp32 values (2^-24 of 1, so u / (1 - b) of those factors): checked
-against the same fp32 coefficients, 8 u of the terms' magnitudes; p moves by lr_t m / (sqrt(v) + eps), off by 16 u of the
+of two products whose four coefficients round to fp32 (the rates come in double), 8 u of the terms' magnitudes; p moves by lr_t m / (sqrt(v) + eps), off by 16 u of the
 step's size, and rounds by u.
 """
 import math
@@ -162,8 +161,7 @@ def test_captured_and_replayed(cuda):
 
 
 def adam64(p, g, m, v, lr, b1, b2, eps, scale, t):
-    b1, b2, eps, lr = (float(torch.tensor(a, dtype=torch.float32)) for a in (b1, b2, eps, lr))
-    c1, c2 = float(torch.tensor(1.0) - torch.tensor(b1)), float(torch.tensor(1.0) - torch.tensor(b2))
+    c1, c2 = 1 - b1, 1 - b2
     g = g.double().cpu() * scale
     m, v = m.double().cpu(), v.double().cpu()
     m2, v2 = b1 * m + c1 * g, b2 * v + c2 * g * g
@@ -291,7 +289,7 @@ def test_trainer_clips_to_the_global_norm(cuda):
     assert norm > 2.0 and torch.equal(free.net.flat_grad, eager.net.flat_grad)
     assert abs(eager.grad_norm.item() - norm) <= 2 * U * norm
     # first step: m = (1 - b1) g'
-    c1 = float(torch.tensor(1.0) - torch.tensor(0.9))
+    c1 = 1 - 0.9
     assert ((eager.m.double() - c1 * g / norm).abs() <= 8 * U * (c1 * g / norm).abs() + 2.0 ** -133).all()
     for _ in range(2):
         eager.step(batch)
