@@ -1135,10 +1135,11 @@ static GnGeom gn_geom(int n, int P, int c, int groups, int V, bool backward) {
     g.rows = g.slots * k;
     g.S = g.R ? ceil_div(g.R, g.rows) : 1;
     g.parts = g.S * g.tiles;
-    // The second launch's cut changes no sum: one block a CU where its fold and table are a good part of the work, several
-    // where the tensor is large, four rows a thread at least.
+    // The second launch's cut changes no sum: one block a CU where its fold and table are a good part of the work, many where
+    // the tensor is large (16 x 1080 x 1920 x 32 bf16, forward: 2048 blocks 1248 us, 4096 1099, 8192 1092), four rows a thread
+    // at least.
     const long mb = (long)n * P * c / V * 16 >> 20;
-    const int blocks2 = mb > 256 ? 2048 : mb > 48 || backward ? 512 : 256;
+    const int blocks2 = mb > 256 ? 8192 : mb > 48 || backward ? 512 : 256;
     const int k2 = ceil_div((long)deep * g.tiles * (n > 0 ? n : 1), blocks2);
     g.rows2 = g.slots * (k2 > 4 ? k2 : 4);
     g.S2 = g.R ? ceil_div(g.R, g.rows2) : 1;
