@@ -95,7 +95,7 @@ __device__ __forceinline__ float gn_dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, 0xf, 0xf, true));
 }
 
-// the sum of an exchange's two results (the elements are copied first: a bit cast of a vector's element reads element 0)
+// the sum of an exchange's two results (copied first: this compiler's bit cast of a vector's element reads element 0)
 __device__ __forceinline__ float gn_add_pair(u32x2 r) {
     const unsigned lo = r[0], hi = r[1];
     return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
@@ -849,7 +849,8 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
 // ------------------------------------------------------------------ small samples: one launch
 // A unit is one group, or the V / D groups of one 16-byte column where D < V; its P pixels x DV columns stay in the
 // registers of ONE block: read once, the mean first, then the deviations from it, then the result.  Neighbouring units
-// share cache lines: the block numbers are dealt so that they run on one XCD (one L2).
+// share cache lines: the block numbers are dealt so that they run on one XCD (one L2): 16 samples of 32 x 32 x 512 bf16 in 32
+// groups 18.5 -> 11.0 us forward, 31.6 -> 19.5 backward.
 struct GnUnit {
     int n, unit, DV, Ta, col, pix, dpix;
     long at;   // the thread's first vector, in elements

@@ -716,6 +716,7 @@ def _chk_here(t, name):
 def _chk_out(out, name, like, *exact):
     """An output buffer of like's shape and type: one of `exact` itself, or no overlap with any of them."""
     _chk(out, name, like.dtype, like.shape)
+    _chk_here(out, name)
     a, size = out.data_ptr(), out.numel() * out.element_size()
     for t in exact:
         if t is not None and t.data_ptr() != a and abs(t.data_ptr() - a) < size:
@@ -742,6 +743,7 @@ def _group_norm_ws(ws, x, groups, backward):
         ws = torch.empty(need, dtype=torch.float32, device=x.device)
     else:
         _chk(ws, 'ws', torch.float32)
+        _chk_here(ws, 'ws')
         if ws.numel() < need or ws.data_ptr() % 16:
             raise ValueError('ws must be 16-byte aligned and hold group_norm_ws_floats(...) = %d floats' % need)
     return ws.data_ptr(), ws
@@ -778,7 +780,7 @@ def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None
     if stats is None:
         stats = torch.empty((n, groups, 2), dtype=torch.float32, device=x.device)
     else:
-        _chk(stats, 'stats', torch.float32, (n, groups, 2))
+        _chk_here(_chk(stats, 'stats', torch.float32, (n, groups, 2)), 'stats')
     _lib.call('stmi_group_norm_nhwc_fwd', x.data_ptr(), wsp, stats.data_ptr(), eps, scale.data_ptr(), shift.data_ptr(),
               _ptr(residual), y.data_ptr(), act, n, h, w, c, groups, _DT[x.dtype], _stream_on(dev))
     return y, stats
@@ -1079,10 +1081,12 @@ def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, s
         _chk(step_dev, 'step_dev', torch.int32)
         t = 0 if advance else -1
     if clip is not None:
-        _chk_here(p, 'p')
         clip._chk_current()
         if norm is not None:
             _chk(norm, 'norm', torch.float32, (1,))
+        for tns, nm in ((p, 'p'), (g, 'g'), (m, 'm'), (v, 'v'), (norm, 'norm'), (step_dev, 'step_dev')):
+            if tns is not None:
+                _chk_here(tns, nm)
         _lib.call('stmi_adam_tf1_clip', p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(), float(lr),
                   float(beta1), float(beta2), float(eps), float(grad_scale), clip._ws_place, clip._n, float(max_norm),
                   _ptr(norm), _ptr(step_dev), int(t), _stream())
