@@ -300,12 +300,14 @@ def test_places(cuda, shape, dtype, form):
         (_, xv), (_, rv), (ybuf, yv), (_, dyv) = (at(t, k) for t, k in zip((x, res, torch.zeros_like(x), dy), places))
         ops.group_norm_fwd(xv, groups, scale, shift, act=ops.ACT_SILU, residual=rv, out=yv)
         near(yv, f['y'], 1.1 * f['dz'] + U * f['y'].abs().max().item(), dtype)
+        assert torch.equal(yv, y)           # a sample's bits do not depend on its place
         k, m = places[2], x.numel()
         assert (ybuf[:k] == 2).all() and (ybuf[k + m:] == 2).all()
         dxbuf, dxv = at(x, places[2])
         gs, gh = torch.zeros((2, dims[3]), device=cuda)
         ops.group_norm_bwd(xv, dyv, groups, st, scale, shift, gs, gh, act=ops.ACT_SILU, out=dxv)
         near(dxv, f['dx'], f['dx_tol'], dtype)
+        assert torch.equal(dxv, dx)
         near(gs, f['dscale'], f['dscale_tol'])
         assert (dxbuf[:k] == 2).all() and (dxbuf[k + m:] == 2).all()
 
