@@ -1183,6 +1183,10 @@ static bool gn_in_units(const GnGeom& g, int V, int most_threads, int* threads, 
     return false;
 }
 
+// Samples of one launch of `units` blocks a sample: a grid has less than 2^32 threads, 131072 samples of one pixel and 4096
+// channels fill it.
+static int gn_unit_samples(int units, int threads) { return (int)((1L << 31) / threads / units); }
+
 long gn_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward) {
     const int V = dtype == STMI_BF16 ? 8 : 4;
     const GnGeom g = gn_geom(n, h * w, c, groups, V, backward);
@@ -1241,13 +1245,18 @@ static int gn_fwd_t(const T* x, float* ws, float* stats, float eps, const float*
     int threads, u;
     if (gn_in_units(g, V, kGnUnitFwd, &threads, &u)) {
         const int wide = g.D > V ? g.D : V;
-        const dim3 grid((unsigned)ceil_div((long)n * (c / wide), 8) * 8);
         g.rQT = gn_recip(wide / V);
-        gn_unit_launch<V, 2>(g, u, [&](auto NS, auto U) {
-            hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads), 0, s, x, stats,
-                               eps, scale, shift, residual, y, act, g);
-        });
-        STMI_LAUNCH_CHECK("gn_unit_fwd_kernel");
+        const int most = gn_unit_samples(c / wide, threads);
+        for (long n0 = 0; n0 < n; n0 += most) {
+            const long at = n0 * P * c;
+            g.N = n - n0 < most ? (int)(n - n0) : most;
+            const dim3 grid((unsigned)ceil_div((long)g.N * (c / wide), 8) * 8);
+            gn_unit_launch<V, 2>(g, u, [&](auto NS, auto U) {
+                hipLaunchKernelGGL((gn_unit_fwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads), 0, s, x + at,
+                                   stats + n0 * groups * 2, eps, scale, shift, residual ? residual + at : nullptr, y + at, act, g);
+            });
+            STMI_LAUNCH_CHECK("gn_unit_fwd_kernel");
+        }
         return STMI_OK;
     }
     return gn_with_form(GnStream(1, residual ? 2 : 1, n, P, c, sizeof(T)), g, [&](auto NT, auto PT, auto TL) -> int {
@@ -1290,15 +1299,21 @@ static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* sc
     int threads, u;
     if (gn_in_units(g, V, kGnUnitBwd, &threads, &u)) {
         const int wide = g.D > V ? g.D : V;
-        const dim3 grid((unsigned)ceil_div((long)n * (c / wide), 8) * 8);
         g.rQT = gn_recip(wide / V);
         g.lgC = gn_lg_lanes(wide, threads);
         float* r = dscale && n > 1 ? ws : nullptr;
-        gn_unit_launch<V, 4>(g, u, [&](auto NS, auto U) {
-            hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads),
-                               2 * V * threads * sizeof(float), s, x, dy, stats, scale, shift, dx, r, dscale, dshift, accumulate, act, g);
-        });
-        STMI_LAUNCH_CHECK("gn_unit_bwd_kernel");
+        const int most = gn_unit_samples(c / wide, threads);
+        for (long n0 = 0; n0 < n; n0 += most) {
+            const long at = n0 * P * c;
+            g.N = n - n0 < most ? (int)(n - n0) : most;
+            const dim3 grid((unsigned)ceil_div((long)g.N * (c / wide), 8) * 8);
+            gn_unit_launch<V, 4>(g, u, [&](auto NS, auto U) {
+                hipLaunchKernelGGL((gn_unit_bwd_kernel<T, V, decltype(NS)::value, decltype(U)::value>), grid, dim3(threads),
+                                   2 * V * threads * sizeof(float), s, x + at, dy + at, stats + n0 * groups * 2, scale, shift, dx + at,
+                                   r ? r + n0 * 2 * c : nullptr, dscale, dshift, accumulate, act, g);
+            });
+            STMI_LAUNCH_CHECK("gn_unit_bwd_kernel");
+        }
         if (r) {
             hipLaunchKernelGGL(gn_param_grads_kernel, dim3(ceil_div(2L * c, 64)), dim3(kGnT), 0, s, (const float*)r, (long)n, dscale,
                                dshift, accumulate, c);

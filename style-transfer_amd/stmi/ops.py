@@ -1003,7 +1003,8 @@ class GradList:
     many there are.  tensors: contiguous fp32 / bf16 tensors of any lengths on the current device; outs: what clip() writes,
     tensor by tensor (default: the tensors themselves).  The list keeps the tensors, their places (a device table built
     here, once) and a workspace: build it before a graph that uses it is captured, keep it as long as the graph and until its
-    work has ended, and order its calls (two graphs that may run at the same time need a list each)."""
+    work has ended, and order its calls (two graphs that may run at the same time need a list each).  The tensors have to
+    stay where they are: one that got other memory since (set_(), resize_(), .data = ..., a new .grad) needs a new list."""
 
     def __init__(self, tensors, outs=None):
         import ctypes

@@ -399,6 +399,29 @@ def test_more_samples_than_a_grid_dimension(cuda, c, groups):
     near(gh, f['dshift'], f['dshift_tol'])
 
 
+def test_more_threads_than_a_grid_dimension(cuda):
+    """One block per group: 131075 samples of 512 groups are more than 2^32 threads.  Seven samples over and over: the batch
+    gives the bits of the seven."""
+    from stmi import ops
+    times, c, groups = 18725, 4096, 512
+    x, scale, shift, dy, _ = (t.to(cuda) for t in data((7, 1, 1, c), torch.bfloat16, 41))
+    many = lambda t: t.repeat(times, 1, 1, 1)   # noqa: E731
+    y, stats = ops.group_norm_fwd(x, groups, scale, shift, eps=EPS)
+    dx = ops.group_norm_bwd(x, dy, groups, stats, scale, shift, None, None)
+    yy, ss = ops.group_norm_fwd(many(x), groups, scale, shift, eps=EPS)
+    assert torch.equal(yy, many(y)) and torch.equal(ss, stats.repeat(times, 1, 1))
+    del yy
+    gs, gh = torch.zeros((2, c), device=cuda)
+    assert torch.equal(ops.group_norm_bwd(many(x), many(dy), groups, ss, scale, shift, gs, gh), many(dx))
+    # a channel's terms are added in eight runs: each addition is off by 2^-24 of what the terms' sizes sum to
+    mean, rstd = (stats[..., k].double().repeat_interleave(c // groups, 1) for k in (0, 1))
+    d = dy.double().view(7, c)
+    terms = d * (x.double().view(7, c) - mean) * rstd
+    for got, t in ((gs, terms), (gh, d)):
+        size = times * t.abs().sum(0)
+        assert ((got.double() - times * t.sum(0)).abs() <= size * 2.0 ** -24 * (7 * times / 8 + 16)).all()
+
+
 def test_empty_batch(cuda):
     from stmi import ops
     x = torch.empty((0, 4, 4, 8), device=cuda)
