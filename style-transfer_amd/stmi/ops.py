@@ -808,6 +808,8 @@ def group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, act=ACT_N
                       (dshift, 'dshift')):
             if t is not None:
                 _chk_here(t, nm)
+    if dscale is not None and abs(dscale.data_ptr() - dshift.data_ptr()) < 4 * c:
+        raise ValueError('dscale and dshift overlap')
     wsp, ws = _group_norm_ws(ws, x, groups, True)
     dx = torch.empty_like(x) if out is None else _chk_out(out, 'out', x, x, dy)
     _lib.call('stmi_group_norm_nhwc_bwd', x.data_ptr(), dy.data_ptr(), stats.data_ptr(), scale.data_ptr(), shift.data_ptr(),

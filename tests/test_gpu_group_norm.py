@@ -435,6 +435,17 @@ def test_empty_batch(cuda):
     assert (gs == 0).all() and (gh == 0).all()
 
 
+def test_parameter_gradients_in_one_place_are_refused(cuda):
+    from stmi import ops
+    x = torch.zeros((2, 4, 4, 8), device=cuda)
+    s, both = torch.ones(8, device=cuda), torch.zeros(16, device=cuda)
+    y, stats = ops.group_norm_fwd(x, 2, s, s)
+    for gs, gh in ((both[:8], both[:8]), (both[:8], both[4:12]), (both[4:12], both[:8])):
+        with pytest.raises(ValueError, match='overlap'):
+            ops.group_norm_bwd(x, x, 2, stats, s, s, gs, gh)
+    ops.group_norm_bwd(x, x, 2, stats, s, s, both[8:], both[:8])   # neighbours are fine
+
+
 def test_refusals(cuda):
     from stmi import lib, ops
     x = torch.zeros((2, 4, 4, 8), device=cuda)
