@@ -467,7 +467,8 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count,
 /* tf.clip_by_global_norm over any number of fp32 / bf16 tensors of any lengths, contiguous, at any element alignment
  * (no call site in the reference, which trains unclipped):
  *   norm = sqrt(sum over all tensors of sum(g^2)),  out = g * max_norm / max(norm, max_norm);
- * a norm that is not finite makes every output NaN.  Squares are summed in double, in a fixed order.
+ * a gradient that is not finite makes every output NaN.  Squares are summed in double, in a fixed order; the norm of finite
+ * gradients may exceed fp32: it is then reported as infinity, and the outputs are clipped by its true value.
  * The tensors are described by a DEVICE table of chunks: stmi_grad_list_chunks gives its length, stmi_grad_list_fill
  * writes it to HOST memory (no launch), the caller copies it to the device and keeps it for as long as the tensors
  * (srcs) and the outputs (dsts, elementwise the same shapes and types; dsts[i] may be srcs[i], no other overlap) stay

@@ -51,11 +51,19 @@ __device__ __forceinline__ double fold_squares(const double* __restrict__ ws, in
     return block_sum_d(v, red);
 }
 
-// max_norm / max(norm, max_norm); NaN where the norm is not finite
-__device__ __forceinline__ float clip_factor(double norm, float max_norm) {
-    if (!(norm <= 1.7976931348623157e308)) return __builtin_nanf("");
-    return norm > (double)max_norm ? (float)((double)max_norm / norm) : 1.f;
-}
+// scale * max_norm / max(norm, max_norm) as a product of two fp32 factors; NaN where the norm is not finite.
+// b is 1 unless the factor is below 2^-120 (norms of finite gradients reach 2^128 and more), too little for one fp32 number.  A
+// normal result then needs |g| > 2^-6, and g * 2^-120 is still a normal number: nothing is lost before the last product.
+struct ClipFactor {
+    float a, b;
+    __device__ __forceinline__ ClipFactor(double norm, float max_norm, double scale) : b(1.f) {
+        const double f = norm > (double)max_norm ? scale * ((double)max_norm / norm) : scale;
+        const bool tiny = fabs(f) < 0x1p-120 && f != 0.0;
+        a = !(norm <= 1.7976931348623157e308) ? __builtin_nanf("") : tiny ? 0x1p-120f : (float)f;
+        if (tiny) b = (float)(f * 0x1p120);
+    }
+    __device__ __forceinline__ float operator()(float g) const { return g * a * b; }
+};
 
 // the vectors of a chunk that thread i owns
 struct Chunk {
@@ -140,10 +148,10 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const stmi_grad_chunk* 
     if (k >= 0) Chunk(table[k]).load(raw);
     const double norm = sqrt(fold_squares(ws, nparts, red));
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
-    const float f = clip_factor(norm, max_norm);
+    const ClipFactor f(norm, max_norm, 1.0);
     for (bool first = true; k >= 0; k -= gridDim.x, first = false) {
         const Chunk ch(table[k]);
-        if (f == 1.f && ch.src == ch.dst) continue;
+        if (f.a == 1.f && ch.src == ch.dst) continue;
         if (!first) ch.load(raw);
 #pragma unroll
         for (int u = 0; u < kVecs; u++) {
@@ -153,14 +161,14 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const stmi_grad_chunk* 
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const unsigned w = raw[u][j];
-                o[j] = ch.half ? bf16_pair(bf16_lo(w) * f, bf16_hi(w) * f) : __builtin_bit_cast(unsigned, __builtin_bit_cast(float, w) * f);
+                o[j] = ch.half ? bf16_pair(f(bf16_lo(w)), f(bf16_hi(w))) : __builtin_bit_cast(unsigned, f(__builtin_bit_cast(float, w)));
             }
             store16<kNt>(ch.dst + i * 16, o);
         }
         const int at = (ch.half ? ch.vecs << 3 : ch.vecs << 2) + threadIdx.x;
         if (at < ch.count) {
-            if (ch.half) ((bf16_t*)ch.dst)[at] = (bf16_t)(to_f32<bf16_t>(((const bf16_t*)ch.src)[at]) * f);
-            else ((float*)ch.dst)[at] = ((const float*)ch.src)[at] * f;
+            if (ch.half) ((bf16_t*)ch.dst)[at] = (bf16_t)f(to_f32<bf16_t>(((const bf16_t*)ch.src)[at]));
+            else ((float*)ch.dst)[at] = f(((const float*)ch.src)[at]);
         }
     }
 }
@@ -212,7 +220,7 @@ int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws,
 }
 
 // ------------------------------------------------------------------ Adam with clipping
-// The update of stmi_adam_tf1 with g' = g * grad_scale * factor, factor from the norm of g * grad_scale: clipping costs
+// The update of stmi_adam_tf1 with g' = g * (grad_scale * factor), factor from the norm of g * grad_scale: clipping costs
 // no pass of its own.  The rates come in double: 1 - beta2 and 1 - beta2^t of an fp32 0.999 are 1.3e-5 off, and the step
 // with them.  28 bytes a parameter; four parameters a thread and access, and the loads of a thread's first ones
 // are on their way while the block folds the partial sums and one thread of its last wave works out the step size.
@@ -250,9 +258,10 @@ __global__ __launch_bounds__(256) void adam_clip_kernel(float* __restrict__ p, c
     const float b1 = (float)beta1, b2 = (float)beta2, c1 = (float)(1.0 - beta1), c2 = (float)(1.0 - beta2);
     const double norm = sqrt(fold_squares(ws, nparts, red)) * fabs((double)grad_scale);   // its barrier is sh's too
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)norm;
-    const float lr_t = sh, gs = grad_scale * clip_factor(norm, max_norm);
+    const float lr_t = sh;
+    const ClipFactor factor(norm, max_norm, grad_scale);
     auto update = [&](float gi, float& mi, float& vi, float& pi) {
-        gi *= gs;
+        gi = factor(gi);
         mi = b1 * mi + c1 * gi;
         vi = b2 * vi + c2 * gi * gi;
         pi -= lr_t * mi / (sqrtf(vi) + eps);

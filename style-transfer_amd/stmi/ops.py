@@ -1059,8 +1059,9 @@ class GradList:
         return out
 
     def clip(self, max_norm, norm=None):
-        """outs = tensors * max_norm / max(norm, max_norm); returns the norm before clipping, fp32 [1] on the device.  A norm
-        that is not finite makes every output NaN."""
+        """outs = tensors * max_norm / max(norm, max_norm); returns the norm before clipping, fp32 [1] on the device.  A
+        gradient that is not finite makes every output NaN; a norm of finite ones beyond fp32 is returned as infinity, and the
+        outputs are clipped by its true value."""
         norm = self._norm_out(norm)
         _lib.call('stmi_grad_clip', self._place, self._n, self._ws_place, float(max_norm), norm.data_ptr(),
                   _stream_on(self._dev))
