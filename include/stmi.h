@@ -367,8 +367,9 @@ int stmi_instance_norm_param_grads(const float* rows, int nrows, int n, int c, f
  * groups == c is the instance norm, groups == 1 normalises a whole picture).  Group k of a sample is its channels
  * k*c/groups .. (k+1)*c/groups - 1 at every pixel; with mean and variance over the group
  *   xhat = (x - mean) / sqrt(var + eps),  y = act(scale[c] * xhat + shift[c]) [+ residual].
- * c must be a multiple of groups and at most STMI_GN_MAX_C, eps at least 1e-30; every STMI_ACT_* activation; NaN and
- * infinities of a group (and deviations whose squares leave fp32, 1e19) make all of that group's outputs NaN and no others.
+ * c must be a multiple of groups and at most STMI_GN_MAX_C, eps at least 1e-30; every STMI_ACT_* activation.  Values may be of
+ * any size, their deviations from the group's mean up to 1e18 (squares are summed in fp32).  NaN and infinities of a group (and
+ * deviations whose squares leave fp32) make all of that group's outputs NaN and no others.
  *
  * fwd : stats[n,groups,2] (fp32) = (mean, 1/sqrt(var + eps)), for the backward pass.  y may be x or residual itself.
  * bwd : from dy (gradient w.r.t. y) to dx, and dscale[c], dshift[c] (fp32; written, or added to what they hold when

@@ -17,8 +17,9 @@
 // on the sample's own size alone, and accesses need only the elements' alignment (global memory takes 16-byte accesses at
 // any address): a sample's bits depend neither on its batch nor on its place.
 // A mean is formed first and deviations from it are summed then, within a batch of loads, over a block's threads and over
-// the slices: no cancellation however large the mean is next to the deviation.  Sums are fp32, no atomics:
-// bit-reproducible.
+// the slices: no cancellation however large the mean is next to the deviation.  Means are themselves sums of deviations, from
+// a value of the group, and every term enters a sum with its weight 1 / M: equal values give their own value and no deviation,
+// and nothing leaves fp32 unless a deviation's square does.  Sums are fp32, no atomics: bit-reproducible.
 // What the launches of small tensors cost is instructions, not bytes: divisions by the geometry's numbers are done by the
 // host (gn_div), constants of the channels come from a table in shared memory that a block makes once, reductions over
 // lanes use DPP.
@@ -224,7 +225,7 @@ __device__ __forceinline__ void gn_column(const float* tab, const GnGeom& g, int
 }
 
 // ------------------------------------------------------------------ forward, first launch
-// ws[n][slice * tiles + tile][G][2]: (mean, sum of squared deviations) of the block's values of each group; their number
+// ws[n][slice * tiles + tile][G][2]: (mean, sum of squared deviations / M) of the block's values of each group; their number
 // follows from the cut (gn_share).
 // A thread keeps a mean and a sum of squared deviations per channel of its column: a batch of kB values is summed as
 // deviations from the mean so far (from the first value in the first batch), then mean += s1 / n, m2 += s2 - s1^2 / n
@@ -238,7 +239,10 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
     extern __shared__ float sh[];   // [V][kGnT] means, [V][kGnT] sums of squares, [kGnT] counts
     const GnPlace<kTiled> p(g, V, g.S, g.rows);
     if (p.n >= g.N) return;
-    float mean[V], m2[V];
+    // the group's first value in the sample, from which the block's means deviate (team of the first round; on its way meanwhile)
+    const T* x0 = x + (long)p.n * g.P * g.C;
+    const float first = to_f32<T>(x0[min((int)threadIdx.x >> g.lgG, g.G - 1) * g.D]);
+    float mean[V], m2[V];   // m2: divided by M
 #pragma unroll
     for (int j = 0; j < V; j++) mean[j] = m2[j] = 0.f;
     int cnt = 0;
@@ -252,7 +256,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
             for (int j = 0; j < V; j++) {
                 const float e = s1[j] * rn;
                 mean[j] += e;
-                m2[j] += s2[j] - s1[j] * e;
+                m2[j] += (s2[j] - s1[j] * e) * g.rM;
             }
         };
         auto add = [&](const u32x4& raw, float (&s1)[V], float (&s2)[V]) {
@@ -306,7 +310,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
             for (int j = 0; j < V; j += 2 * w) {
                 const float d = mean[j + w] - mean[j];
                 mean[j] += 0.5f * d;
-                m2[j] += m2[j + w] + d * d * (0.5f * (float)(cnt * w));
+                m2[j] += m2[j + w] + d * d * (0.5f * (float)(cnt * w) * g.rM);
             }
         }
     }
@@ -319,7 +323,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
         lm[j * kGnT + threadIdx.x] = mean[j];
         l2[j * kGnT + threadIdx.x] = m2[j];
     }
-    lc[threadIdx.x] = (float)(cnt * g.U);
+    lc[threadIdx.x] = (float)(cnt * g.U) * g.rM;   // the entry's share of the group
     __syncthreads();
     // a team of lanes adds the entries of one group up, the means first, then the deviations from their mean
     const int K = 1 << g.lgG, lane = threadIdx.x & (K - 1);
@@ -329,7 +333,8 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
     for (int gr0 = 0; gr0 < g.G; gr0 += kGnT >> g.lgG) {
         const int gr = gr0 + (threadIdx.x >> g.lgG);
         const bool live = gr < g.G;
-        // f(count, mean, sum of squared deviations) of every entry of the group
+        const float from = gr0 == 0 ? first : live ? to_f32<T>(x0[gr * g.D]) : 0.f;
+        // f(share, mean, sum of squared deviations / M) of every entry of the group
         auto each = [&](auto f) {
             for (int en = en0; en < entries; en += enstep) {
                 const int rep = gn_div(en, g.rUnits);
@@ -342,14 +347,14 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
             }
             if (g.tail && p.last) {
                 for (int e = lane; e < g.tail / g.C * g.D; e += K)
-                    f(1.f, to_f32<T>(x[p.end0 + e / g.D * g.C + gr * g.D + e % g.D]), 0.f);
+                    f(g.rM, to_f32<T>(x[p.end0 + e / g.D * g.C + gr * g.D + e % g.D]), 0.f);
             }
         };
         float n = 0.f, s1 = 0.f, s2 = 0.f;
-        if (live) each([&](float c, float m, float) { n += c; s1 += c * m; });
+        if (live) each([&](float c, float m, float) { n += c; s1 += c > 0.f ? c * (m - from) : 0.f; });
         n = gn_team_sum(n, g.lgG);
         s1 = gn_team_sum(s1, g.lgG);
-        const float mu = n > 0.f ? s1 / n : 0.f;
+        const float mu = n > 0.f ? from + s1 / n : from;
         if (live) each([&](float c, float m, float q) { const float d = c > 0.f ? m - mu : 0.f; s2 += q + c * d * d; });
         s2 = gn_team_sum(s2, g.lgG);
         if (live && lane == 0) out[gr] = make_float2(mu, s2);
@@ -371,7 +376,7 @@ __device__ __forceinline__ float gn_share(const GnGeom& g, int gr, int i) {
 }
 
 // (mean, 1/sqrt(var + eps)) of group gr of sample n from its partials, NK at most a lane of the team, in two passes: the
-// mean first, then the deviations from it.  Every lane ends with the result.
+// mean first (from the first partial's), then the deviations from it.  Every lane ends with the result.
 template <int NK, bool kTiled>
 __device__ __forceinline__ void gn_fold_n(const float2* __restrict__ w, const GnGeom& g, int gr, int lg, float eps, float& mean,
                                           float& rstd) {
@@ -379,17 +384,18 @@ __device__ __forceinline__ void gn_fold_n(const float2* __restrict__ w, const Gn
     float2 r[NK];
 #pragma unroll
     for (int k = 0; k < NK; k++) r[k] = w[(unsigned)(min(lane + (k << lg), g.parts - 1) * g.G)];
+    const float from = w[0].x;
     float share[NK], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < NK; k++) {
         share[k] = gn_share<kTiled>(g, gr, lane + (k << lg));
-        s1 += share[k] > 0.f ? share[k] * r[k].x : 0.f;
+        s1 += share[k] > 0.f ? share[k] * (r[k].x - from) : 0.f;
     }
-    mean = gn_team_sum(s1, lg);
+    mean = from + gn_team_sum(s1, lg);
 #pragma unroll
     for (int k = 0; k < NK; k++) {
         const float d = r[k].x - mean;
-        s2 += share[k] > 0.f ? r[k].y * g.rM + share[k] * d * d : 0.f;
+        s2 += share[k] > 0.f ? r[k].y + share[k] * d * d : 0.f;
     }
     rstd = gn_rsqrt(gn_team_sum(s2, lg) + eps);
 }
@@ -907,6 +913,8 @@ __global__ __launch_bounds__(1024) void gn_unit_fwd_kernel(const T* x, float* __
     for (int u = 0; u < kU; u++)
         if (u_.pix + u * u_.dpix < g.P) raw[u] = gn_load<false>(x + u_.at + u * step, 0);
     const int c0 = u_.unit * max(g.D, V) + u_.col * V;
+    // the unit's first 16 bytes: its groups' first values, from which the mean deviates
+    const u32x4 first = gn_load<false>(x + ((long)u_.n * g.P * g.C + (long)u_.unit * max(g.D, V)), 0);
     float a[V], b[V];
     if (u_.pix < g.P) {
 #pragma unroll
@@ -916,7 +924,8 @@ __global__ __launch_bounds__(1024) void gn_unit_fwd_kernel(const T* x, float* __
         }
     }
     const float rM = g.rM;
-    float mean[NS], rstd[NS];
+    float x0[V], mean[NS], rstd[NS];
+    gn_unpack<T, V>(first, x0);
 #pragma unroll
     for (int k = 0; k < NS; k++) mean[k] = rstd[k] = 0.f;
 #pragma unroll
@@ -925,12 +934,12 @@ __global__ __launch_bounds__(1024) void gn_unit_fwd_kernel(const T* x, float* __
             float v[V];
             gn_unpack<T, V>(raw[u], v);
 #pragma unroll
-            for (int j = 0; j < V; j++) mean[j / W] += v[j];
+            for (int j = 0; j < V; j++) mean[j / W] += (v[j] - x0[j / W * W]) * rM;
         }
     }
     gn_block_sums<NS>(mean, red);
 #pragma unroll
-    for (int k = 0; k < NS; k++) mean[k] *= rM;
+    for (int k = 0; k < NS; k++) mean[k] += x0[k * W];
 #pragma unroll
     for (int u = 0; u < kU; u++) {
         if (u_.pix + u * u_.dpix < g.P) {
@@ -939,14 +948,14 @@ __global__ __launch_bounds__(1024) void gn_unit_fwd_kernel(const T* x, float* __
 #pragma unroll
             for (int j = 0; j < V; j++) {
                 const float d = v[j] - mean[j / W];
-                rstd[j / W] += d * d;
+                rstd[j / W] += d * rM * d;
             }
         }
     }
     gn_block_sums<NS>(rstd, red);
 #pragma unroll
     for (int k = 0; k < NS; k++) {
-        rstd[k] = gn_rsqrt(rstd[k] * rM + eps);
+        rstd[k] = gn_rsqrt(rstd[k] + eps);
         if (threadIdx.x == 0) {
             float* st = stats + ((long)u_.n * g.G + u_.unit * NS + k) * 2;
             st[0] = mean[k];
@@ -1049,7 +1058,7 @@ __global__ __launch_bounds__(512) void gn_unit_bwd_kernel(const T* x, const T* d
 #pragma unroll
         for (int k = 0; k < NS; k++) {
             m[k] *= rM;
-            m[NS + k] *= rM * rstd[k] * rstd[k];
+            m[NS + k] = m[NS + k] * rM * rstd[k] * rstd[k];   // in this order: the product alone may be below 2^-126
         }
 #pragma unroll
         for (int u = 0; u < kU; u++) {
