@@ -716,22 +716,28 @@ __global__ __launch_bounds__(kGnT) void gn_fold_sums_kernel(const float2* __rest
     }
 }
 
-// dshift / dscale from the partial rows: outputs o of [0, 2C), 64 a block, eight row groups each, in one fixed order
+// dshift / dscale from the partial rows: outputs o of [0, 2C), 64 a block, eight row groups each, in one fixed order.  Added in
+// double: thousands of samples make long runs (131075 equal terms in fp32 were 1.6e-4 off, now 2e-8).  tmp: a number a thread
 __device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, long nrows, float* __restrict__ dscale,
-                                               float* __restrict__ dshift, int accumulate, int C, int block, float* tmp) {
+                                               float* __restrict__ dshift, int accumulate, int C, int block, double* tmp) {
     const int o = block * 64 + (threadIdx.x & 63), rg = threadIdx.x >> 6;
-    float s = 0.f;
+    double s = 0.0;
     if (o < 2 * C) {
+        long i = rg;
+        for (; i + 15 * (kGnT / 64) < nrows; i += 16 * (kGnT / 64)) {
+#pragma unroll
+            for (int u = 0; u < 16; u++) s += rows[(i + u * (kGnT / 64)) * 2 * C + o];
+        }
 #pragma unroll 8
-        for (long i = rg; i < nrows; i += kGnT / 64) s += rows[i * 2 * C + o];
+        for (; i < nrows; i += kGnT / 64) s += rows[i * 2 * C + o];
     }
     tmp[threadIdx.x] = s;
     __syncthreads();
     if (rg == 0 && o < 2 * C) {
-        s = 0.f;
+        s = 0.0;
         for (int k = 0; k < kGnT / 64; k++) s += tmp[k * 64 + threadIdx.x];
         float* dst = o < C ? dshift + o : dscale + (o - C);
-        *dst = accumulate ? *dst + s : s;
+        *dst = accumulate ? *dst + (float)s : (float)s;
     }
 }
 
@@ -747,12 +753,13 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
                                                             int accumulate, int act, const GnGeom g) {
     constexpr int kU = 2;
     // [5][C] mean, scale * rstd, shift, k1 = rstd m1, k2 = rstd^2 m2 with dx = scale rstd g - k1 - (x - mean) k2; [2G] m1, m2
-    // (512 floats at least)
+    // (512 doubles at least)
     extern __shared__ float tab[];
     const int blocks2 = g.S2 * g.tiles;
     if ((int)blockIdx.x >= blocks2) {
         const long q = (long)(blockIdx.x - blocks2) * g.N + gn_sample();
-        if (gn_sample() < g.N && q * 64 < 2 * g.C) gn_param_grads(rows, (long)g.N * g.parts, dscale, dshift, accumulate, g.C, (int)q, tab);
+        if (gn_sample() < g.N && q * 64 < 2 * g.C)
+            gn_param_grads(rows, (long)g.N * g.parts, dscale, dshift, accumulate, g.C, (int)q, (double*)tab);
         return;
     }
     const GnPlace<kTiled> p(g, V, g.S2, g.rows2);
@@ -1104,7 +1111,7 @@ __global__ __launch_bounds__(512) void gn_unit_bwd_kernel(const T* x, const T* d
 
 __global__ __launch_bounds__(kGnT) void gn_param_grads_kernel(const float* __restrict__ rows, long nrows, float* dscale,
                                                               float* dshift, int accumulate, int C) {
-    __shared__ float tmp[kGnT];
+    __shared__ double tmp[kGnT];
     gn_param_grads(rows, nrows, dscale, dshift, accumulate, C, blockIdx.x, tmp);
 }
 
@@ -1347,7 +1354,7 @@ static int gn_bwd_t(const T* x, const T* dy, const float* stats, const float* sc
             STMI_LAUNCH_CHECK("gn_fold_sums_kernel");
             m = msums;
         }
-        const int pblocks = dscale ? ceil_div(2L * c, 64) : 0, table = 5 * c + 2 * groups > kGnT ? 5 * c + 2 * groups : kGnT;
+        const int pblocks = dscale ? ceil_div(2L * c, 64) : 0, table = 5 * c + 2 * groups > 2 * kGnT ? 5 * c + 2 * groups : 2 * kGnT;
         STMI_DYN_LDS((gn_bwd_apply_kernel<T, V, kNt, kPut, kTiled>), 7 * STMI_GN_MAX_C * (int)sizeof(float), "gn_bwd_apply_kernel");
         hipLaunchKernelGGL((gn_bwd_apply_kernel<T, V, kNt, kPut, kTiled>), gn_grid(g.S2 * g.tiles + ceil_div(pblocks, n), n), dim3(kGnT),
                            table * sizeof(float), s, x, dy, stats, scale, shift, (const float2*)grows, m, (const float*)rows, dx, dscale,

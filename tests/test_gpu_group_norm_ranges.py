@@ -55,3 +55,45 @@ def test_deviations_up_to_the_stated_size(cuda, shape, mean, form):
     # dx is of the size of 1e-18: its terms are formed from numbers above 2^-126, k2 = rstd^2 m2 (1e-36) to 2^-149
     bound['dx'] = bound['dx'] + 2.0 ** -148 * 1e18
     assert not B.faults({'y': y, 'dx': dx, 'dshift': dshift, 'dscale': dscale}, want, bound, parts, torch.float32)
+
+
+@pytest.mark.parametrize('shape', [(40000, 2, 3, 8, 2), (5000, 4, 4, 64, 8), (3000, 3, 3, 35, 5)], ids=B.name)
+def test_parameter_gradients_of_large_batches(cuda, shape, form):
+    """The samples' partial sums (bounds of one sample) are added up without further loss: one rounding of the result."""
+    from stmi import ops
+    *dims, groups = shape
+    gen = torch.Generator().manual_seed(5)
+    n, h, w, c = dims
+    x, scale, shift = torch.randn(dims, generator=gen).to(cuda), torch.ones(c, device=cuda), torch.zeros(c, device=cuda)
+    # equal terms: in a running sum of 32 bits their roundings do not cancel
+    dy = torch.full(dims, 0.7, device=cuda)
+    _, stats = ops.group_norm_fwd(x, groups, scale, shift, eps=B.EPS)
+    dscale, dshift = torch.zeros((2, c), device=cuda)
+    ops.group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, accumulate=False)
+    want = dy.double().sum((0, 1, 2))
+    # a sample's h w terms: at most h w roundings of at most u of the partial sum
+    assert ((dshift.double() - want).abs() <= (h * w + 1) * U * want.abs()).all()
+    mean, rstd = (stats[..., k].double().repeat_interleave(c // groups, 1).view(n, 1, 1, c) for k in (0, 1))
+    terms = dy.double() * (x.double() - mean) * rstd
+    assert ((dscale.double() - terms.sum((0, 1, 2))).abs() <= ((h * w + 6) * U * terms.abs().sum((0, 1, 2)))).all()
+
+
+def test_parameter_gradients_of_the_samples_behind_the_first_launch(cuda):
+    """131075 samples of 512 groups take several launches of one block per group.  Only the samples at their borders have
+    gradients: a row that is lost or counted twice shows in full."""
+    from stmi import ops
+    n, c, groups = 131075, 4096, 512
+    x7, scale, shift, dy7 = (t.to(cuda) for t in B.data((7, 1, 1, c), groups, torch.bfloat16, 41))
+    x = x7.repeat(18725, 1, 1, 1)
+    dy = torch.zeros_like(x)
+    at = [0, 1, 65535, 65536, 131070, 131071, 131072, 131073, 131074]
+    for k, i in enumerate(at):
+        dy[i] = dy7[k % 7]
+    _, stats = ops.group_norm_fwd(x, groups, scale, shift, eps=B.EPS)
+    dscale, dshift = torch.zeros((2, c), device=cuda)
+    dx = ops.group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, accumulate=False)
+    few_x, few_dy = x[at].contiguous(), dy[at].contiguous()
+    want, parts = B.results(few_x, groups, scale, shift, ops.ACT_NONE, few_dy)
+    assert not B.faults({'dx': dx[at], 'dscale': dscale, 'dshift': dshift}, want, B.bounds(parts), parts, torch.bfloat16)
+    dx[at] = 0
+    assert not dx.any()
