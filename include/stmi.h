@@ -474,7 +474,8 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count,
  * writes it to HOST memory (no launch), the caller copies it to the device and keeps it for as long as the tensors
  * (srcs) and the outputs (dsts, elementwise the same shapes and types; dsts[i] may be srcs[i], no other overlap) stay
  * where they are.  Tensors of length zero have no chunks.
- * ws: STMI_GRAD_WS_DOUBLES doubles of scratch.  Calls that share a ws must be ordered.
+ * ws: STMI_GRAD_WS_DOUBLES doubles of scratch.  Calls that share a ws must be ordered.  A clip that overwrites its own tensors
+ * leaves the partial sums of what they were: stmi_grad_sum_squares again before stmi_adam_tf1_clip.
  * stmi_grad_sum_squares : leaves partial sums of squares in ws for stmi_adam_tf1_clip.
  * stmi_grad_norm        : the same, and norm (device fp32 [1]).
  * stmi_grad_clip        : the same, and the outputs; norm (may be NULL) is the norm BEFORE clipping.  Where dsts[i] is

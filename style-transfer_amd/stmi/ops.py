@@ -1006,7 +1006,10 @@ class GradList:
     tensor by tensor (default: the tensors themselves).  The list keeps the tensors, their places (a device table built
     here, once) and a workspace: build it before a graph that uses it is captured, keep it as long as the graph and until its
     work has ended, and order its calls (two graphs that may run at the same time need a list each).  The tensors have to
-    stay where they are: one that got other memory since (set_(), resize_(), .data = ..., a new .grad) needs a new list."""
+    stay where they are: one that got other memory since (set_(), resize_(), .data = ..., a new .grad) needs a new list.
+    sum_squares(), norm() and clip() leave the tensors' norm for adam_tf1(clip=), each new set of gradients needs one of
+    them; after a clip() that overwrites them the norm is no longer theirs.  (The list knows of the calls that are made, not of
+    those that a graph replays.)"""
 
     def __init__(self, tensors, outs=None):
         import ctypes
@@ -1033,8 +1036,11 @@ class GradList:
                   (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts, dtypes, n, table)
         self._table = torch.frombuffer(table, dtype=torch.uint8).to(self.device)
         self._place = self._table.data_ptr()
-        self._ws = torch.empty(_lib.GRAD_WS_DOUBLES, dtype=torch.float64, device=self.device)
+        # NaN: a norm that no launch has left (one that was captured and not replayed yet) makes the update NaN
+        self._ws = torch.full((_lib.GRAD_WS_DOUBLES,), float('nan'), dtype=torch.float64, device=self.device)
         self._ws_place = self._ws.data_ptr()
+        self._in_place = any(o.data_ptr() == t.data_ptr() for t, o in zip(tensors, outs) if t.numel())
+        self._summed = False     # the workspace holds the norm of the tensors as the last call of this list left them
 
     def _chk_current(self):
         if torch.cuda.current_device() != self._dev:
@@ -1051,11 +1057,13 @@ class GradList:
         """Leaves the sum of squares (as partial sums) for adam_tf1(..., clip=self)."""
         self._chk_current()
         _lib.call('stmi_grad_sum_squares', self._place, self._n, self._ws_place, _stream_on(self._dev))
+        self._summed = True
 
     def norm(self, out=None):
         """The global L2 norm, fp32 [1] on the device."""
         out = self._norm_out(out)
         _lib.call('stmi_grad_norm', self._place, self._n, self._ws_place, out.data_ptr(), _stream_on(self._dev))
+        self._summed = True
         return out
 
     def clip(self, max_norm, norm=None):
@@ -1065,6 +1073,7 @@ class GradList:
         norm = self._norm_out(norm)
         _lib.call('stmi_grad_clip', self._place, self._n, self._ws_place, float(max_norm), norm.data_ptr(),
                   _stream_on(self._dev))
+        self._summed = not self._in_place
         return norm
 
 
@@ -1074,10 +1083,12 @@ def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, s
     """TF1 Adam.  With `step_dev` (int32 [1] on the device) the step number lives on the device, which
     makes the call replayable inside a HIP graph: advance=True increments it before use; advance=False
     uses it as it stands (a second slice of the same parameter set in the same step).
-    clip: a GradList whose sum_squares() has been launched; the gradients g * grad_scale are then clipped to the global
-    norm max_norm on their way in, with |grad_scale| times the list's norm (fp32 [1] `norm` receives it)."""
+    clip: a GradList whose sum_squares() has been launched for these gradients; g * grad_scale is then clipped to the global
+    norm max_norm on its way in, with |grad_scale| times the list's norm (fp32 [1] `norm` receives it)."""
     if (clip is None) != (max_norm is None) or (clip is None and norm is not None):
         raise ValueError('clip and max_norm are given together, norm with them')
+    if clip is not None and not clip._summed and 0 < max_norm < float('inf'):   # another max_norm is refused by the call below
+        raise ValueError('the list holds no norm of its tensors: call sum_squares() before the update')
     for tns, nm in ((p, 'p'), (g, 'g'), (m, 'm'), (v, 'v')):
         _chk(tns, nm, torch.float32)
         assert tns.numel() == p.numel()
