@@ -727,6 +727,9 @@ int stmi_adam_tf1(float* p, const float* g, float* m, float* v, long count, floa
     return adam_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, step_dev, t, S(stream));
 }
 
+// the kernels' int index of a chunk runs past the last one by at most the STMI_GRAD_WS_DOUBLES blocks of a grid
+static const long kMostChunks = (1L << 31) - 4096;
+
 long stmi_grad_list_chunks(const long* counts, const int* dtypes, int n) {
     if (n < 0 || (n > 0 && !(counts && dtypes))) return -1;
     for (int i = 0; i < n; i++)
@@ -745,24 +748,24 @@ int stmi_grad_list_fill(const void* const* srcs, void* const* dsts, const long* 
     }
     const long chunks = grad_list_chunks(counts, dtypes, n);
     STMI_REQUIRE(chunks == 0 || host_table, "grad_list_fill: null table");
-    STMI_REQUIRE(chunks < (1L << 31), "grad_list_fill: more than 2^31 chunks");
+    STMI_REQUIRE(chunks <= kMostChunks, "grad_list_fill: more than 2^31 - 2^12 chunks");
     grad_list_fill(srcs, dsts, counts, dtypes, n, host_table);
     return STMI_OK;
 }
 
 int stmi_grad_sum_squares(const stmi_grad_chunk* table, int nchunks, double* ws, void* stream) {
-    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws, "grad_sum_squares: bad arguments");
+    STMI_REQUIRE(nchunks >= 0 && nchunks <= kMostChunks && (table || nchunks == 0) && ws, "grad_sum_squares: bad arguments");
     return grad_squares_impl(table, nchunks, ws, S(stream));
 }
 
 int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float* norm, void* stream) {
-    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws && norm, "grad_norm: bad arguments");
+    STMI_REQUIRE(nchunks >= 0 && nchunks <= kMostChunks && (table || nchunks == 0) && ws && norm, "grad_norm: bad arguments");
     const int rc = grad_squares_impl(table, nchunks, ws, S(stream));
     return rc ? rc : grad_norm_impl(ws, nchunks, norm, S(stream));
 }
 
 int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream) {
-    STMI_REQUIRE(nchunks >= 0 && (table || nchunks == 0) && ws, "grad_clip: bad arguments");
+    STMI_REQUIRE(nchunks >= 0 && nchunks <= kMostChunks && (table || nchunks == 0) && ws, "grad_clip: bad arguments");
     STMI_REQUIRE(max_norm > 0.f && max_norm <= 3.402823466e38f, "grad_clip: max_norm must be finite and > 0 (got %g)", (double)max_norm);
     const int rc = grad_squares_impl(table, nchunks, ws, S(stream));
     return rc ? rc : grad_scale_impl(table, nchunks, ws, max_norm, norm, S(stream));
@@ -771,7 +774,7 @@ int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float 
 int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count, double lr, double beta1, double beta2,
                        float eps, float grad_scale, const double* ws, int nchunks, float max_norm, float* norm, int* step_dev,
                        int t, void* stream) {
-    STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws && nchunks >= 0, "adam_tf1_clip: bad arguments");
+    STMI_REQUIRE(count >= 0 && (count == 0 || (p && g && m && v)) && ws && nchunks >= 0 && nchunks <= kMostChunks, "adam_tf1_clip: bad arguments");
     STMI_REQUIRE(step_dev || t >= 1, "adam_tf1_clip: step t must be >= 1 (got %d)", t);
     STMI_REQUIRE(max_norm > 0.f && max_norm <= 3.402823466e38f, "adam_tf1_clip: max_norm must be finite and > 0 (got %g)", (double)max_norm);
     return adam_clip_impl(p, g, m, v, count, lr, beta1, beta2, eps, grad_scale, ws, nchunks, max_norm, norm, step_dev, t, S(stream));
