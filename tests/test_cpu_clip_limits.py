@@ -20,3 +20,11 @@ def test_lists_whose_index_would_overflow_are_refused():
         assert h.stmi_grad_norm(1, n, 1, 1, None) == -1
         assert h.stmi_grad_clip(1, n, 1, 1.0, 1, None) == -1
         assert h.stmi_adam_tf1_clip(1, 1, 1, 1, 8, 1e-3, .9, .999, 1e-8, 1.0, 1, n, 1.0, None, None, 1, None) == -1
+
+
+def test_outputs_beside_the_tensors_are_taken():
+    import torch
+    from stmi.ops import _chk_disjoint
+    a, b = torch.zeros(100), torch.zeros(100)
+    _chk_disjoint([a], [b])
+    _chk_disjoint([a[:50], b[50:]], [a[50:], b[:50]])
