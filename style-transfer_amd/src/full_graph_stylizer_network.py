@@ -287,7 +287,7 @@ def _tail_trainer(cache, main, n, vgg_weights, vgg_mean, style_config, dtype):
     if n not in cache:
         t = StyleTrainer(n, main.h, main.w, main.device, vgg_weights, vgg_mean, style_config.style_weight,
                          style_config.content_weight, style_config.total_variation_weight, dtype=dtype, lr=main.lr,
-                         use_graph=False)
+                         use_graph=False, max_grad_norm=main.max_grad_norm)
         t.style_targets = main.style_targets
         cache[n] = t
     t = cache[n]
@@ -298,6 +298,8 @@ def _tail_trainer(cache, main, n, vgg_weights, vgg_mean, style_config, dtype):
 
 def _sync_back(tail, main):
     main.net.flat.copy_(tail.net.flat); main.m.copy_(tail.m); main.v.copy_(tail.v); main.step_dev.copy_(tail.step_dev)
+    if main.grad_norm is not None:
+        main.grad_norm.copy_(tail.grad_norm)
     main.net.repack()
 
 
