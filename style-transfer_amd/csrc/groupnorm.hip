@@ -351,7 +351,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
             }
         };
         float n = 0.f, s1 = 0.f, s2 = 0.f;
-        if (live) each([&](float c, float m, float) { n += c; s1 += c > 0.f ? c * (m - from) : 0.f; });
+        if (live) each([&](float c, float m, float) { n += c; s1 += c * (m - from); });
         n = gn_team_sum(n, g.lgG);
         s1 = gn_team_sum(s1, g.lgG);
         const float mu = n > 0.f ? from + s1 / n : from;
