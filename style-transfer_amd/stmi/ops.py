@@ -1032,14 +1032,14 @@ class GradList:
         dtypes = (ctypes.c_int * n)(*[_DT[t.dtype] for t in tensors])
         self._n = h.stmi_grad_list_chunks(counts, dtypes, n)
         table = (_lib.GradChunk * max(self._n, 1))()
-        _lib.call('stmi_grad_list_fill', (ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-                  (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs]), counts, dtypes, n, table)
+        src, dst = [t.data_ptr() for t in tensors], [o.data_ptr() for o in outs]
+        _lib.call('stmi_grad_list_fill', (ctypes.c_void_p * n)(*src), (ctypes.c_void_p * n)(*dst), counts, dtypes, n, table)
         self._table = torch.frombuffer(table, dtype=torch.uint8).to(self.device)
         self._place = self._table.data_ptr()
         # NaN: a norm that no launch has left (one that was captured and not replayed yet) makes the update NaN
         self._ws = torch.full((_lib.GRAD_WS_DOUBLES,), float('nan'), dtype=torch.float64, device=self.device)
         self._ws_place = self._ws.data_ptr()
-        self._in_place = any(o.data_ptr() == t.data_ptr() for t, o in zip(tensors, outs) if t.numel())
+        self._in_place = any(a == b and a for a, b in zip(src, dst))   # tensors of length zero are nowhere
         self._summed = False     # the workspace holds the norm of the tensors as the last call of this list left them
 
     def _chk_current(self):
