@@ -376,6 +376,7 @@ int stmi_instance_norm_param_grads(const float* rows, int nrows, int n, int c, f
  *       accumulate != 0; both NULL: not computed), summed over samples in a fixed order.  dx may be x or dy itself.  The
  *       gradient w.r.t. residual is dy.  With n == 0, dscale and dshift are zero (left as they are when accumulated).
  * ws  : scratch of stmi_group_norm_ws_floats floats for the direction, 16-byte aligned (NULL where that is 0).
+ * Outputs (y, stats, dx, dscale, dshift, ws) overlap nothing else but as stated here.
  * No float atomics: results are bit-reproducible, and a sample's result does not depend on the batch it is part of. */
 #define STMI_GN_MAX_C 4096
 long stmi_group_norm_ws_floats(int n, int h, int w, int c, int groups, int dtype, int backward);
@@ -494,7 +495,8 @@ int stmi_grad_norm(const stmi_grad_chunk* table, int nchunks, double* ws, float*
 int stmi_grad_clip(const stmi_grad_chunk* table, int nchunks, double* ws, float max_norm, float* norm, void* stream);
 /* stmi_adam_tf1 of gradients clipped on the way in: g * grad_scale is scaled by max_norm / max(norm, max_norm) with
  * norm = |grad_scale| * sqrt(sum of the partial sums in ws), as stmi_grad_sum_squares left them for all gradients that
- * share the norm (nchunks: that call's).  norm (device fp32 [1], may be NULL) receives it. */
+ * share the norm (nchunks: that call's).  norm (device fp32 [1], may be NULL) receives it.  The rates are doubles here and
+ * fp32 in stmi_adam_tf1 (1 - 0.999 is 1.3e-5 off there): where nothing is clipped the two updates differ by that much. */
 int stmi_adam_tf1_clip(float* p, const float* g, float* m, float* v, long count,
                        double lr, double beta1, double beta2, float eps, float grad_scale,
                        const double* ws, int nchunks, float max_norm, float* norm, int* step_dev, int t, void* stream);

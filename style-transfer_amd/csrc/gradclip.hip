@@ -93,7 +93,7 @@ __device__ __forceinline__ unsigned bf16_pair(float lo, float hi) {
     return w;
 }
 
-// 600 tensors, 112 MB: 18.5 us, 6.0 TB/s
+// 600 tensors, 112 MB: 21 us, 5.2 TB/s
 __global__ __launch_bounds__(256) void grad_squares_kernel(const stmi_grad_chunk* __restrict__ table, int nchunks,
                                                            double* __restrict__ ws) {
     __shared__ double red[4];
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const double* __restrict
 
 // The chunks are taken from the last to the first: what grad_squares_kernel read last is the likeliest to be in a cache
 // still.  The loads of a block's first chunk are on their way while it folds the partial sums.
-// 600 tensors, 223 MB read and written: 35 us, 6.4 TB/s
+// 600 tensors, 223 MB read and written: 36 us, 6.2 TB/s
 template <bool kNt>
 __global__ __launch_bounds__(256) void grad_scale_kernel(const stmi_grad_chunk* __restrict__ table, int nchunks,
                                                          const double* __restrict__ ws, int nparts, float max_norm,
@@ -222,9 +222,9 @@ int grad_scale_impl(const stmi_grad_chunk* table, int nchunks, const double* ws,
 // ------------------------------------------------------------------ Adam with clipping
 // The update of stmi_adam_tf1 with g' = g * (grad_scale * factor), factor from the norm of g * grad_scale: clipping costs
 // no pass of its own.  The rates come in double: 1 - beta2 and 1 - beta2^t of an fp32 0.999 are 1.3e-5 off, and the step
-// with them.  28 bytes a parameter; four parameters a thread and access, and the loads of a thread's first ones
+// with them.  (stmi_adam_tf1 keeps fp32 rates: the two updates agree to 1.3e-5 where nothing is clipped, not to the bit.)  28 bytes a parameter; four parameters a thread and access, and the loads of a thread's first ones
 // are on their way while the block folds the partial sums and one thread of its last wave works out the step size.
-// 20 M parameters (561 MB): 92 us, 6.1 TB/s with the gradients still cached; 1.7 M (47 MB) 9.5 us.
+// 20 M parameters (561 MB): 95 us, 5.9 TB/s with the gradients still cached; 1.7 M (47 MB) 12 us.
 
 // b^t for t >= 0 by squaring: t times 2^-53 off at most, and shorter than two pow()
 __device__ __forceinline__ double pow_int(double b, unsigned t) {

@@ -231,8 +231,8 @@ __device__ __forceinline__ void gn_column(const float* tab, const GnGeom& g, int
 // deviations from the mean so far (from the first value in the first batch), then mean += s1 / n, m2 += s2 - s1^2 / n
 // with n the count behind the batch.  That shift is a value of the plane or a mean of some, so s2 exceeds the sum it
 // stands for by no more than the batch's share of the total, and the short batches keep partial sums short.
-// Bound by reading: 16 x 1080 x 1920 x 32 bf16 (2.1 GB) in 300 us, 7.1 TB/s; 4 x 256 x 256 x 32 (17 MB) 5.6 us, of which about
-// 4 are start, first latency and reductions.
+// Bound by reading: 16 x 1080 x 1920 x 32 bf16 (2.1 GB) in 312 us, 6.8 TB/s; 4 x 256 x 256 x 32 (17 MB) in 7.0 us, 5.4 where the
+// tensor is in the last-level cache: 256 blocks, a block's loads, reductions and partial result one after the other.
 template <typename T, int V, bool kNt, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ ws, const GnGeom g) {
     constexpr int kB = 8;
@@ -429,7 +429,7 @@ __global__ __launch_bounds__(kGnT) void gn_fold_kernel(const float2* __restrict_
 // A slice is walked from its end: what the first launch read last is the likeliest to be in a cache still.  The loads of a
 // thread's first rows are on their way while the block folds the partials and makes its table (mean, scale * rstd, shift of
 // every channel), those of the next rows while it computes.
-// 16 x 1080 x 1920 x 32 bf16 (4.2 GB read and written): 790 us, 5.4 TB/s, a copy's rate; 4 x 256 x 256 x 32 7.2 us.
+// 16 x 1080 x 1920 x 32 bf16 (4.2 GB read and written): 778 us, 5.5 TB/s, a copy's rate; 4 x 256 x 256 x 32 (34 MB) 7.2 us.
 template <typename T, int V, bool kNt, bool kPut, bool kRes, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const float2* __restrict__ ws, float* __restrict__ stats,
                                                         float eps, const float* __restrict__ scale,
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_apply_kernel(const T* x, const flo
 // ------------------------------------------------------------------ backward, first launch
 // rows[n][slice * tiles + tile][2][C]: the block's sums of g and of g * xhat per channel (the parameter gradients' parts);
 // grows[...][G][2]: the same times scale, per group.  (A thread adds few values: 32 of a 1080p plane.)
-// 4 x 1080 x 1920 x 32 bf16 with SiLU (1.06 GB): 185 us, 5.7 TB/s; its derivative costs an exponential and a reciprocal a value,
+// 4 x 1080 x 1920 x 32 bf16 with SiLU (1.06 GB): 199 us, 5.3 TB/s; its derivative costs an exponential and a reciprocal a value,
 // 12 instructions in all, about half of what the vector units could issue in that time.
 template <typename T, int V, bool kNt, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_bwd_sums_kernel(const T* __restrict__ x, const T* __restrict__ dy,
@@ -744,7 +744,7 @@ __device__ __forceinline__ void gn_param_grads(const float* __restrict__ rows, l
 // ------------------------------------------------------------------ backward, second launch
 // The last blocks fold the parameter gradients, the others write dx.  As in the forward pass a slice is walked from its
 // end, and loads are on their way during the fold and the computation of the rows before.
-// 4 x 1080 x 1920 x 32 bf16 with SiLU (1.6 GB): 285 us, 5.6 TB/s.
+// 4 x 1080 x 1920 x 32 bf16 with SiLU (1.6 GB): 287 us, 5.5 TB/s.
 template <typename T, int V, bool kNt, bool kPut, bool kTiled>
 __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const T* dy, const float* __restrict__ stats,
                                                             const float* __restrict__ scale, const float* __restrict__ shift,
@@ -869,7 +869,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_bwd_apply_kernel(const T* x, const
 // A unit is one group, or the V / D groups of one 16-byte column where D < V; its P pixels x DV columns stay in the
 // registers of ONE block: read once, the mean first, then the deviations from it, then the result.  Neighbouring units
 // share cache lines: the block numbers are dealt so that they run on one XCD (one L2): 16 samples of 32 x 32 x 512 bf16 in 32
-// groups 18.5 -> 11.0 us forward, 31.6 -> 19.5 backward.  One launch of 1 x 16 x 16 x 512 takes 4.5 us, bound by latency.
+// groups 18.5 -> 11.0 us forward, 31.6 -> 19.5 backward.  One launch of 1 x 16 x 16 x 512 takes 4.4 us, bound by latency.
 struct GnUnit {
     int n, unit, DV, Ta, col, pix, dpix;
     long at;   // the thread's first vector, in elements

@@ -762,7 +762,7 @@ def _plain(t, dev, dtype, shape):
 def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None, out=None, stats=None, eps=IN_EPS):
     """y = act(scale * xhat + shift) [+ residual], normalised over `groups` groups of neighbouring channels of x [n,h,w,c].
     Returns (y, stats); stats [n,groups,2] = (mean, 1/sqrt(var+eps)) for group_norm_bwd.  out may be x or residual itself;
-    any other overlap is not allowed.  act: ACT_NONE, ACT_RELU, ACT_SIGMOID or ACT_SILU."""
+    any other overlap (of out, stats or ws with anything) is not allowed.  act: ACT_NONE, ACT_RELU, ACT_SIGMOID or ACT_SILU."""
     n, h, w, c = x.shape
     dev = torch.cuda.current_device() if x.is_cuda else -1
     if not (_plain(x, dev, x.dtype, x.shape) and dev >= 0 and _plain(scale, dev, torch.float32, (c,))
@@ -789,7 +789,7 @@ def group_norm_fwd(x, groups, scale, shift, act=ACT_NONE, residual=None, ws=None
 def group_norm_bwd(x, dy, groups, stats, scale, shift, dscale, dshift, act=ACT_NONE, ws=None, out=None, accumulate=True):
     """dx returned; parameter gradients are ADDED into dscale/dshift (fp32 [c]), or WRITTEN when accumulate is False;
     both None: not computed.  stats: what group_norm_fwd returned for x.  The gradient of a residual is dy.  out may be x or
-    dy itself; any other overlap is not allowed."""
+    dy itself; any other overlap (of out, dscale, dshift or ws with anything) is not allowed."""
     n, h, w, c = x.shape
     if (dscale is None) != (dshift is None):
         raise ValueError('dscale and dshift are given together or not at all')
@@ -1084,7 +1084,8 @@ def adam_tf1(p, g, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, grad_scale=1.0, s
     makes the call replayable inside a HIP graph: advance=True increments it before use; advance=False
     uses it as it stands (a second slice of the same parameter set in the same step).
     clip: a GradList whose sum_squares() has been launched for these gradients; g * grad_scale is then clipped to the global
-    norm max_norm on its way in, with |grad_scale| times the list's norm (fp32 [1] `norm` receives it)."""
+    norm max_norm on its way in, with |grad_scale| times the list's norm (fp32 [1] `norm` receives it).  The clipped update takes
+    its rates in double, the plain one in fp32: with a max_norm that is never reached they differ by up to 1.3e-5 of a step."""
     if (clip is None) != (max_norm is None) or (clip is None and norm is not None):
         raise ValueError('clip and max_norm are given together, norm with them')
     if clip is not None and not clip._summed and 0 < max_norm < float('inf'):   # another max_norm is refused by the call below
