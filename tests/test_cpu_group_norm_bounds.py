@@ -47,3 +47,26 @@ def test_bounds_tell_right_from_wrong(shape, dtype):
     if P <= 512:
         last = B.results(*args, lost=slice(P - 1, P))[0]
         assert seen(last, 'dx') and seen(last, 'dshift') and seen(last, 'dscale')
+
+
+@pytest.mark.parametrize('act', ['NONE', 'RELU', 'SIGMOID', 'SILU'])
+@pytest.mark.parametrize('shape', [(2, 5, 7, 12, 3), (1, 3, 2, 8, 8), (3, 4, 4, 6, 1)], ids=B.name)
+def test_the_formula_is_the_derivative(shape, act):
+    """dx, dscale and dshift of the formula against automatic differentiation of its y, in 64 bits, and against the central
+    difference of sum(dy y) along a random direction: h^2 = 1e-8 of the third derivative, and 1e-16 / h of the sum."""
+    from stmi import ops
+    act = getattr(ops, 'ACT_' + act)
+    *dims, groups = shape
+    x, scale, shift, dy = (t.double() for t in B.data(dims, groups, torch.float32, 9))
+    x = x * 3
+    got, parts = B.results(x, groups, scale, shift, act, dy)
+    leaves = [t.clone().requires_grad_(True) for t in (x, scale, shift)]
+    want = torch.autograd.grad(B.results(leaves[0], groups, leaves[1], leaves[2], act, dy)[0]['y'], leaves, dy.reshape(got['y'].shape))
+    for a, b in zip((got['dx'], got['dscale'], got['dshift']), want):
+        assert (a.reshape(b.shape) - b).abs().max() <= 1e-12 * (1 + b.abs().max())
+    h, gen = 1e-4, torch.Generator().manual_seed(1)
+    assert act != ops.ACT_RELU or parts['z'].abs().min() > 10 * h      # no kink within the difference
+    way = [torch.randn(t.shape, generator=gen).double() * 0.1 for t in (x, scale, shift)]
+    loss = lambda t: (B.results(x + t * way[0], groups, scale + t * way[1], shift + t * way[2], act, dy)[0]['y'] * dy.reshape(got['y'].shape)).sum().item()   # noqa: E731
+    terms = [a.reshape(b.shape) * b for a, b in zip((got['dx'], got['dscale'], got['dshift']), way)]
+    assert abs((loss(h) - loss(-h)) / (2 * h) - sum(t.sum().item() for t in terms)) <= 1e-6 * sum(t.abs().sum().item() for t in terms)
