@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kGnT, 4) void gn_stats_kernel(const T* __restrict__
     extern __shared__ float sh[];   // [V][kGnT] means, [V][kGnT] sums of squares, [kGnT] counts
     const GnPlace<kTiled> p(g, V, g.S, g.rows);
     if (p.n >= g.N) return;
-    // the group's first value in the sample, from which the block's means deviate (team of the first round; on its way meanwhile)
+    // the group's first value in the sample, from which the block's means deviate: on its way during the sums
     const T* x0 = x + (long)p.n * g.P * g.C;
     const float first = to_f32<T>(x0[min((int)threadIdx.x >> g.lgG, g.G - 1) * g.D]);
     float mean[V], m2[V];   // m2: divided by M
